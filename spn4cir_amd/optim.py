@@ -50,10 +50,11 @@ class AdamW(torch.optim.Optimizer):
         self._step_dev = None               # 0-dim fp32 device counter of APPLIED steps (shared by every state["step"])
 
     # -------------------------------------------------------------------------------- layout
-    def _build_plans(self, members):
-        """members: per group a list of (parameter, m, v) (moments None for 8 bits) -> one AdamWPlan for each 16 groups.  Parameters
-        that share memory (tied weights held twice) are updated one after the other, each by a plan of its own."""
-        self._plans = []
+    def _make_plans(self, members):
+        """members: per group a list of (parameter, m, v) (moments None for 8 bits) -> [(AdamWPlan, its parameters, its groups)], one for
+        each 16 groups.  Parameters that share memory (tied weights held twice) are updated one after the other, each by a plan of its own.
+        Nothing of the optimizer changes here: a plan that cannot be built (out of memory) leaves it as it was."""
+        plans = []
         for g0 in range(0, len(members), ADAMW_GROUPS):
             part = [(i, t) for i, group in enumerate(members[g0:g0 + ADAMW_GROUPS]) for t in group]
             if not part:
@@ -62,7 +63,8 @@ class AdamW(torch.optim.Optimizer):
             for some in ([t] for t in part) if tied else (part,):
                 state = None if self.state_bits == 8 else [(m, v) for _, (_, m, v) in some]
                 plan = AdamWPlan([p for _, (p, _, _) in some], state_bits=self.state_bits, groups=[i for i, _ in some], state=state)
-                self._plans.append((plan, [p for _, (p, _, _) in some], self.param_groups[g0:g0 + ADAMW_GROUPS]))
+                plans.append((plan, [p for _, (p, _, _) in some], self.param_groups[g0:g0 + ADAMW_GROUPS]))
+        return plans
 
     def _build_8bit(self):
         ps = [[p for p in g["params"] if p.requires_grad] for g in self.param_groups]
@@ -70,14 +72,14 @@ class AdamW(torch.optim.Optimizer):
         for p in (p for g in ps for p in g):
             if p.dtype != torch.float32 or not p.is_cuda or not p.is_contiguous():
                 raise TypeError("spn4cir_amd.optim.AdamW: parameters must be contiguous fp32 CUDA tensors")
-        self._step_dev = torch.zeros((), dtype=torch.float32, device=dev)
-        self._build_plans([[(p, None, None) for p in g] for g in ps])
-        for plan, params, _ in self._plans:
+        step_dev = torch.zeros((), dtype=torch.float32, device=dev)
+        plans = self._make_plans([[(p, None, None) for p in g] for g in ps])
+        for plan, params, _ in plans:
             for p, off, n in zip(params, plan.offsets, plan.numels):
-                st, end = self.state[p], off + (n + 127) // 128 * 128
-                st["step"] = self._step_dev
-                st["exp_avg"], st["exp_avg_sq"] = plan.m[off:end], plan.v[off:end]
-                st["exp_avg_scale"], st["exp_avg_sq_scale"] = plan.m_scale[off // 128:end // 128], plan.v_scale[off // 128:end // 128]
+                end = off + (n + 127) // 128 * 128
+                self.state[p].update(step=step_dev, exp_avg=plan.m[off:end], exp_avg_sq=plan.v[off:end],
+                                     exp_avg_scale=plan.m_scale[off // 128:end // 128], exp_avg_sq_scale=plan.v_scale[off // 128:end // 128])
+        self._plans, self._step_dev = plans, step_dev        # (last: a failed build is tried again by the next step)
 
     @staticmethod
     def _own_grad(p):
@@ -92,8 +94,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("state_bits=8: add all parameters before the first step")
         super().add_param_group(param_group)
 
-    def _step_plans(self, grads_of, scale, found, exact_betas):
-        """One adamw_multi per plan; grads_of(p) -> its gradient or None."""
+    def _refresh_plans(self):
         for k, (plan, params, groups) in enumerate(self._plans):
             if list(map(torch.Tensor.data_ptr, params)) != plan.addresses:       # p.data was replaced: the moments stay, the addresses do not
                 state = plan.own_moments if self.state_bits == 32 else (plan.m, plan.v, plan.m_scale, plan.v_scale)
@@ -101,16 +102,22 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("a parameter changed its size after the first step")
                 plan = AdamWPlan(params, state_bits=self.state_bits, groups=plan.groups, state=state)
                 self._plans[k] = (plan, params, groups)
+
+    def _plan_calls(self, grads_of, exact_betas):
+        """[(plan, gradients, hyper-parameters)] of one adamw_multi per plan; grads_of(p) -> its gradient or None."""
+        calls = []
+        for plan, params, groups in self._plans:
             grads = [grads_of(p) for p in params]
             if all(g is None for g in grads):
                 continue
-            hyper = [dict(g, betas=g["betas"] if exact_betas else tuple(C.c_float(b).value for b in g["betas"])) for g in groups]
-            adamw_multi(plan, grads, 0, hyper, seed=self.seed, step_dev=self._step_dev, grad_scale=scale, found_inf=found)
+            calls.append((plan, grads, [dict(g, betas=g["betas"] if exact_betas else tuple(C.c_float(b).value for b in g["betas"]))
+                                        for g in groups]))
+        return calls
 
     def _build_runs(self):
-        self._runs = []
+        all_runs = []
         dev = next(p.device for g in self.param_groups for p in g["params"])
-        self._step_dev = torch.zeros((), dtype=torch.float32, device=dev)
+        step_dev = torch.zeros((), dtype=torch.float32, device=dev)
         for group in self.param_groups:
             ps = [p for p in group["params"] if p.requires_grad]
             for p in ps:
@@ -133,15 +140,15 @@ class AdamW(torch.optim.Optimizer):
                 n = sum(p.numel() for p in r)
                 m = torch.zeros(n, dtype=torch.float32, device=r[0].device)
                 v = torch.zeros(n, dtype=torch.float32, device=r[0].device)
-                off = 0
-                for p in r:                                  # torch-compatible per-parameter state (views of the run's state)
-                    st = self.state[p]
-                    st["step"] = self._step_dev
-                    st["exp_avg"] = m[off:off + p.numel()].view_as(p)
-                    st["exp_avg_sq"] = v[off:off + p.numel()].view_as(p)
-                    off += p.numel()
                 out.append(dict(params=r, p_flat=_flat_view(r[0], n), m=m, v=v, numel=n))
-            self._runs.append(out)
+            all_runs.append(out)
+        for run in (run for runs in all_runs for run in runs):
+            off = 0
+            for p in run["params"]:                          # torch-compatible per-parameter state (views of the run's state)
+                end = off + p.numel()
+                self.state[p].update(step=step_dev, exp_avg=run["m"][off:end].view_as(p), exp_avg_sq=run["v"][off:end].view_as(p))
+                off = end
+        self._runs, self._step_dev = all_runs, step_dev      # (last: a failed build is tried again by the next step)
 
     def load_state_dict(self, state_dict):
         """torch semantics; the loaded per-parameter moments are copied into the flat state of the runs."""
@@ -216,12 +223,13 @@ class AdamW(torch.optim.Optimizer):
         for t in (scale, found):
             if t is not None and (t.dtype != torch.float32 or not t.is_cuda or t.numel() != 1):
                 raise TypeError("grad_scale / found_inf must be 1-element fp32 CUDA tensors")
-        check(lib().spn_adamw_tick(_p(self._step_dev), _p(found), _stream()), "adamw_tick")
+        # everything that can fail for want of memory or a wrong layout is done before the step is counted and the first kernel launched
         if self.state_bits == 8:
-            self._step_plans(self._own_grad, scale, found, True)
+            self._refresh_plans()
+            launches, calls = [], self._plan_calls(self._own_grad, True)
             touched = {p.untyped_storage().data_ptr(): p for _, params, _ in self._plans for p in params}.values()      # one of each buffer
         else:
-            touched, loose = [], set()
+            touched, loose, launches, calls = [], set(), [], []          # launches: (p, g, m, v, group)
             one_by_one = self._plans is None and torch.cuda.is_current_stream_capturing()      # a plan's upload cannot be captured
             for group, runs in zip(self.param_groups, self._runs):
                 for run in runs:
@@ -229,24 +237,31 @@ class AdamW(torch.optim.Optimizer):
                         continue
                     g = self._grads_flat(run) if len(run["params"]) > 1 else None
                     if g is not None:
-                        self._launch(run["p_flat"], g, run["m"], run["v"], group, scale, found)
+                        launches.append((run["p_flat"], g, run["m"], run["v"], group))
                     elif one_by_one:
                         off = 0
                         for p in run["params"]:
                             g, n = p.grad, p.numel()
                             if g is not None:
-                                self._launch(_flat_view(p, n), g.contiguous().float().view(-1), run["m"][off:off + n], run["v"][off:off + n],
-                                             group, scale, found)
+                                launches.append((_flat_view(p, n), g.contiguous().float().view(-1), run["m"][off:off + n], run["v"][off:off + n],
+                                                 group))
                             off += n
                     else:                                    # a tensor by itself, or gradients elsewhere: all such in one launch
                         loose.update(run["params"])
                     touched.append(run["params"][0])
             if loose:
                 if self._plans is None:
-                    self._build_plans([[(p, self.state[p]["exp_avg"].view(-1), self.state[p]["exp_avg_sq"].view(-1)) for run in runs
-                                        for p in run["params"]] for runs in self._runs])
+                    self._plans = self._make_plans([[(p, self.state[p]["exp_avg"].view(-1), self.state[p]["exp_avg_sq"].view(-1)) for run in runs
+                                                     for p in run["params"]] for runs in self._runs])
+                else:
+                    self._refresh_plans()
                 # (betas as the single-tensor kernel takes them, in fp32: a tensor's update does not depend on which of the two serves it)
-                self._step_plans(lambda p: self._own_grad(p) if p in loose else None, scale, found, False)
+                calls = self._plan_calls(lambda p: self._own_grad(p) if p in loose else None, False)
+        check(lib().spn_adamw_tick(_p(self._step_dev), _p(found), _stream()), "adamw_tick")
+        for p, g, m, v, group in launches:
+            self._launch(p, g, m, v, group, scale, found)
+        for plan, grads, hyper in calls:
+            adamw_multi(plan, grads, 0, hyper, seed=self.seed, step_dev=self._step_dev, grad_scale=scale, found_inf=found)
         for p in touched:
             p.view(-1)[:0].zero_()                           # bump the buffer's version counter: the models re-derive
                                                              # their bf16 operands when it has moved

@@ -1,0 +1,109 @@
+"""Host logic of spn4cir_amd.optim.AdamW on the CPU: the device calls are stand-ins that count and move the parameters by one."""
+import pytest
+import torch
+
+from spn4cir_amd import optim as O
+
+HP = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.02)
+
+
+class OnGpu(torch.nn.Parameter):
+    """A host tensor that says it lies on the GPU."""
+    is_cuda = property(lambda self: True)
+
+
+class Plan:
+    def __init__(self, params, state_bits=32, groups=None, state=None):
+        self.params, self.state_bits, self.groups, self.own_moments = params, state_bits, groups, state
+        self.addresses, self.numels = [p.data_ptr() for p in params], [p.numel() for p in params]
+        at, self.offsets = 0, []
+        for n in self.numels:
+            self.offsets.append(at)
+            at += (n + 127) // 128 * 128
+        if state_bits == 8:
+            self.m, self.v, self.m_scale, self.v_scale = state or [torch.zeros(k, dtype=torch.uint8) for k in (at, at, at // 128, at // 128)]
+
+
+class Device:
+    """What the stand-ins saw: `fail`: plans that raise before one is built, `ticks`, `calls` = (plan, gradients, hyper) of each launch."""
+
+    def __init__(self):
+        self.fail, self.ticks, self.calls, self.capturing, self.singles = 0, 0, [], False, 0
+
+    def plan(self, *args, **kwargs):
+        if self.fail:
+            self.fail -= 1
+            raise torch.OutOfMemoryError("stand-in")
+        return Plan(*args, **kwargs)
+
+    def multi(self, plan, grads, step, hyper, **kwargs):
+        self.calls.append((plan, grads, hyper))
+        for p, g in zip(plan.params, grads):
+            if g is not None:
+                p.data.add_(1.0)
+
+    def spn_adamw_tick(self, *args):
+        self.ticks += 1
+        return 0
+
+    def spn_adamw_step_dev(self, *args):
+        self.singles += 1
+        return 0
+
+
+@pytest.fixture
+def device(monkeypatch):
+    d = Device()
+    monkeypatch.setattr(O, "AdamWPlan", d.plan)
+    monkeypatch.setattr(O, "adamw_multi", d.multi)
+    monkeypatch.setattr(O, "lib", lambda: d)
+    monkeypatch.setattr(O, "_stream", lambda: None)
+    monkeypatch.setattr(O, "_p", lambda t: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: d.capturing)
+    return d
+
+
+def make(n=4):
+    ps = [OnGpu(torch.zeros(5 + i)) for i in range(n)]
+    for p in ps:
+        p.grad = torch.ones(p.numel())
+    return ps
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("groups,before", [(1, 1), (20, 1), (20, 2)])
+def test_a_failed_first_step_is_not_the_end(device, bits, groups, before):
+    """The construction of the first or second of the plans raises once: that step counts nothing and updates nothing, the next one updates
+    every parameter."""
+    ps = make(groups)
+    o = O.AdamW([dict(params=[p]) for p in ps], state_bits=bits, **HP)
+    real = device.plan
+    made = []
+
+    def plan(*args, **kwargs):
+        made.append(1)
+        if len(made) == before:
+            raise torch.OutOfMemoryError("stand-in")
+        return real(*args, **kwargs)
+    O.AdamWPlan = plan
+    with pytest.raises(torch.OutOfMemoryError):
+        o.step()
+    assert device.ticks == 0 and not device.calls and not any(bool(p.any()) for p in ps)
+    for k in (1.0, 2.0):
+        o.step()
+        assert device.ticks == k and all(bool((p == k).all()) for p in ps)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_failed_rebuild_is_not_the_end(device, bits):
+    """The same for a plan that is rebuilt because a parameter's data was replaced."""
+    ps = make()
+    o = O.AdamW(ps, state_bits=bits, **HP)
+    o.step()
+    ps[1].data = ps[1].data.clone()
+    device.fail = 1
+    with pytest.raises(torch.OutOfMemoryError):
+        o.step()
+    assert device.ticks == 1 and len(device.calls) == 1
+    o.step()
+    assert device.ticks == 2 and all(bool((p == 2).all()) for p in ps) and ps[1].data_ptr() in device.calls[-1][0].addresses
