@@ -20,8 +20,12 @@ parameter list; their gradients may be bf16 or fp16.
 
 state_bits=8 keeps both moments in 8 bits (2.02 instead of 8 bytes per parameter; ops.AdamWPlan): all parameters of all groups go through
 spn_adamw_multi in one launch, whatever buffers they live in.  The moments are rounded stochastically by a hash of (seed, step, element),
-so equal runs give equal bits.  state_dict() holds codes and scale bytes."""
+so equal runs give equal bits.  state_dict() holds codes and scale bytes.
+
+In a graph: init_state() or one step() first, then capture step().  A 32-bit first step that is captured all the same records the creation of its
+state, so that every replay is a first step (with a warning); an 8-bit one is refused, its tables cannot be uploaded there."""
 import ctypes as C
+import warnings
 
 import torch
 
@@ -210,14 +214,26 @@ class AdamW(torch.optim.Optimizer):
                                        float(group["eps"]), float(group["weight_decay"]), _p(self._step_dev), _p(scale),
                                        _p(found), _stream()), "adamw_step_dev")
 
+    def init_state(self):
+        """Creates the moments (zeros), the step counter and the tables of 8-bit moments, which the first step() does otherwise.  A program that captures
+        step() in a graph without a step before it calls this first: what a capture creates is created again by every replay."""
+        if self._step_dev is None:
+            self._build_8bit() if self.state_bits == 8 else self._build_runs()
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        capturing = torch.cuda.is_current_stream_capturing()
         if self._step_dev is None:
-            self._build_8bit() if self.state_bits == 8 else self._build_runs()
+            if capturing and self.state_bits == 8:
+                raise RuntimeError("state_bits=8: call init_state() (or take one step) before step() is captured in a graph")
+            if capturing:
+                warnings.warn("AdamW: the first step is being captured, so the graph zeroes the moments and the step counter too and every replay is a "
+                              "first step; call init_state() (or take one step) before the capture", stacklevel=4)
+            self.init_state()
         scale = getattr(self, "grad_scale", None)          # set by torch.amp.GradScaler.step around this call
         found = getattr(self, "found_inf", None)
         for t in (scale, found):
@@ -230,7 +246,7 @@ class AdamW(torch.optim.Optimizer):
             touched = {p.untyped_storage().data_ptr(): p for _, params, _ in self._plans for p in params}.values()      # one of each buffer
         else:
             touched, loose, launches, calls = [], set(), [], []          # launches: (p, g, m, v, group)
-            one_by_one = self._plans is None and torch.cuda.is_current_stream_capturing()      # a plan's upload cannot be captured
+            one_by_one = self._plans is None and capturing                # a plan's upload cannot be captured
             for group, runs in zip(self.param_groups, self._runs):
                 for run in runs:
                     if all(p.grad is None for p in run["params"]):

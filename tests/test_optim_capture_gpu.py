@@ -1,0 +1,77 @@
+"""spn4cir_amd.optim.AdamW.step() in a graph: replays train as eager steps do."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+HP = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.02)
+SHAPES = [(37, 16), (16,), (64, 130), (5,), (1,), (4100, 3)]
+
+
+@pytest.fixture(scope="module")
+def optim():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from spn4cir_amd import optim as o
+    return o
+
+
+def make(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(s, generator=g).cuda()) for s in SHAPES]
+
+
+def groups(ps):
+    return [dict(params=ps[0::2]), dict(params=ps[1::2], weight_decay=0.0, lr=3e-3)]
+
+
+def gradients(ps, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(p.shape, generator=g) * 0.1).cuda() for p in ps]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("warm", ["init_state", "step"])
+def test_replays_train(optim, bits, warm):
+    """Captured after init_state(), or after a step; then replays with other gradients and eager work between them: the parameters and moments
+    of as many eager steps."""
+    a, b = make(), make()
+    oa, ob = optim.AdamW(groups(a), state_bits=bits, **HP), optim.AdamW(groups(b), state_bits=bits, **HP)
+    for p, q, x in zip(a, b, gradients(a, 0)):
+        p.grad, q.grad = x.clone(), x.clone()
+    done = 0
+    if warm == "init_state":
+        oa.init_state()
+    else:
+        oa.step(), ob.step()
+        done = 1
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oa.step()
+    for t in range(5):
+        for p, q, x in zip(a, b, gradients(a, 1 + t)):
+            p.grad.copy_(x), q.grad.copy_(x)
+        torch.cuda.synchronize()
+        graph.replay()
+        ob.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), t
+        assert float(oa.state[a[0]]["step"]) == done + t + 1
+    for p, q in zip(a, b):
+        assert all(torch.equal(oa.state[p][k], ob.state[q][k]) for k in ("exp_avg", "exp_avg_sq"))
+
+
+def test_an_8_bit_first_step_under_capture_is_refused(optim):
+    """The refusal leaves the optimizer as it was: the next step is the eager first one."""
+    a, b = make(), make()
+    oa, ob = optim.AdamW(groups(a), state_bits=8, **HP), optim.AdamW(groups(b), state_bits=8, **HP)
+    for p, q, x in zip(a, b, gradients(a, 0)):
+        p.grad, q.grad = x.clone(), x.clone()
+    graph, other = torch.cuda.CUDAGraph(), torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        other.add_(1.0)
+        with pytest.raises(RuntimeError, match="init_state"):
+            oa.step()
+    oa.step(), ob.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and float(oa.state[a[0]]["step"]) == 1.0

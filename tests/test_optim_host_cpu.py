@@ -1,4 +1,6 @@
 """Host logic of spn4cir_amd.optim.AdamW on the CPU: the device calls are stand-ins that count and move the parameters by one."""
+import warnings
+
 import pytest
 import torch
 
@@ -107,3 +109,31 @@ def test_a_failed_rebuild_is_not_the_end(device, bits):
     assert device.ticks == 1 and len(device.calls) == 1
     o.step()
     assert device.ticks == 2 and all(bool((p == 2).all()) for p in ps) and ps[1].data_ptr() in device.calls[-1][0].addresses
+
+
+def test_a_first_step_under_capture(device):
+    """8 bits: refused before anything is built or counted, and the next step outside works.  32 bits: a warning (the graph would zero the state
+    at every replay).  After init_state() neither."""
+    ps = make()
+    o = O.AdamW(ps, state_bits=8, **HP)
+    device.capturing = True
+    with pytest.raises(RuntimeError, match="init_state"):
+        o.step()
+    assert device.ticks == 0 and not device.calls and not o.state
+    device.capturing = False
+    o.step()
+    assert device.ticks == 1 and all(bool((p == 1).all()) for p in ps)
+    device.capturing = True
+    with pytest.warns(UserWarning, match="init_state"):
+        O.AdamW(make(), **HP).step()
+    for bits in (8, 32):
+        o = O.AdamW(make(), state_bits=bits, **HP)
+        device.capturing = False
+        o.init_state()
+        state = {p: dict(st) for p, st in o.state.items()}
+        o.init_state()
+        device.capturing = True
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            o.step()
+        assert all(o.state[p][k] is t for p, st in state.items() for k, t in st.items())
