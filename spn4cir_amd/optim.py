@@ -243,9 +243,8 @@ class AdamW(torch.optim.Optimizer):
         if self.state_bits == 8:
             self._refresh_plans()
             launches, calls = [], self._plan_calls(self._own_grad, True)
-            touched = {p.untyped_storage().data_ptr(): p for _, params, _ in self._plans for p in params}.values()      # one of each buffer
         else:
-            touched, loose, launches, calls = [], set(), [], []          # launches: (p, g, m, v, group)
+            loose, launches, calls = set(), [], []           # launches: (p, g, m, v, group)
             one_by_one = self._plans is None and capturing                # a plan's upload cannot be captured
             for group, runs in zip(self.param_groups, self._runs):
                 for run in runs:
@@ -264,7 +263,6 @@ class AdamW(torch.optim.Optimizer):
                             off += n
                     else:                                    # a tensor by itself, or gradients elsewhere: all such in one launch
                         loose.update(run["params"])
-                    touched.append(run["params"][0])
             if loose:
                 if self._plans is None:
                     self._plans = self._make_plans([[(p, self.state[p]["exp_avg"].view(-1), self.state[p]["exp_avg_sq"].view(-1)) for run in runs
@@ -278,9 +276,9 @@ class AdamW(torch.optim.Optimizer):
             self._launch(p, g, m, v, group, scale, found)
         for plan, grads, hyper in calls:
             adamw_multi(plan, grads, 0, hyper, seed=self.seed, step_dev=self._step_dev, grad_scale=scale, found_inf=found)
-        for p in touched:
-            p.view(-1)[:0].zero_()                           # bump the buffer's version counter: the models re-derive
-                                                             # their bf16 operands when it has moved
+        # the version counter of every parameter that was updated: autograd's check of saved tensors and the models, which re-derive their bf16
+        # operands when it has moved, read it (parameters over one buffer need not share a counter)
+        torch.autograd.graph.increment_version([p for group in self.param_groups for p in group["params"] if p.grad is not None and p in self.state])
         if self._on_step is not None:
             self._on_step()
         return loss

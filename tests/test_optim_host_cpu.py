@@ -137,3 +137,35 @@ def test_a_first_step_under_capture(device):
             warnings.simplefilter("error")
             o.step()
         assert all(o.state[p][k] is t for p, st in state.items() for k, t in st.items())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_every_updated_parameter_gets_a_new_version(device, bits):
+    """Parameters re-pointed into one buffer (p.data = a slice) share memory but not a counter; one without a gradient, a frozen one and what the
+    optimizer never touched keep theirs."""
+    ps, flat = make(5), torch.zeros(64)
+    for i, p in enumerate(ps[:3]):
+        p.data = flat[i * 16:(i + 1) * 16]
+        p.grad = torch.ones(16)
+    ps[3].grad = None
+    ps[4].requires_grad_(False)
+    o = O.AdamW(ps, state_bits=bits, **HP)
+    for _ in range(2):
+        before = [p._version for p in ps]
+        o.step()
+        assert [p._version > v for p, v in zip(ps, before)] == [True, True, True, False, False]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_views_of_one_buffer_bump_the_buffer(device, bits):
+    """The models' form: parameters that are views of one flat tensor; its counter moves with theirs, also where one gradient buffer serves all."""
+    flat, grad = torch.zeros(64), torch.ones(64)
+    ps = [OnGpu(flat[i * 16:(i + 1) * 16]) for i in range(4)]
+    for i, p in enumerate(ps):
+        p.grad = grad[i * 16:(i + 1) * 16]
+    o = O.AdamW(ps, state_bits=bits, **HP)
+    for _ in range(2):
+        before = flat._version
+        o.step()
+        assert flat._version > before
+    assert device.singles == (2 if bits == 32 else 0)
