@@ -23,7 +23,8 @@ spn_adamw_multi in one launch, whatever buffers they live in.  The moments are r
 so equal runs give equal bits.  state_dict() holds codes and scale bytes.
 
 In a graph: init_state() or one step() first, then capture step().  A 32-bit first step that is captured all the same records the creation of its
-state, so that every replay is a first step (with a warning); an 8-bit one is refused, its tables cannot be uploaded there."""
+state, so that every replay is a first step (with a warning); an 8-bit one is refused, its tables cannot be uploaded there.  Keep the optimizer as long as
+such a graph; load_state_dict() and p.data = ... give the optimizer new memory, which a graph captured before does not know."""
 import ctypes as C
 import warnings
 
@@ -52,6 +53,7 @@ class AdamW(torch.optim.Optimizer):
         self._on_step = on_step             # e.g. model.parameters_changed (the models also notice the update themselves)
         self._runs = None                   # per group: [dict(params, p_flat, m, v, numel)]
         self._step_dev = None               # 0-dim fp32 device counter of APPLIED steps (shared by every state["step"])
+        self._captured = []                 # what captured steps read and write: kept as long as the optimizer, their graphs hold addresses only
 
     # -------------------------------------------------------------------------------- layout
     def _make_plans(self, members):
@@ -97,6 +99,10 @@ class AdamW(torch.optim.Optimizer):
         if getattr(self, "_step_dev", None) is not None and self.state_bits == 8:
             raise ValueError("state_bits=8: add all parameters before the first step")
         super().add_param_group(param_group)
+
+    def _moved(self):
+        """Whether a parameter's data was replaced since the plans were built."""
+        return any(list(map(torch.Tensor.data_ptr, params)) != plan.addresses for plan, params, _ in self._plans)
 
     def _refresh_plans(self):
         for k, (plan, params, groups) in enumerate(self._plans):
@@ -241,11 +247,13 @@ class AdamW(torch.optim.Optimizer):
                 raise TypeError("grad_scale / found_inf must be 1-element fp32 CUDA tensors")
         # everything that can fail for want of memory or a wrong layout is done before the step is counted and the first kernel launched
         if self.state_bits == 8:
+            if capturing and self._moved():
+                raise RuntimeError("state_bits=8: a parameter's data was replaced; take one step before step() is captured in a graph")
             self._refresh_plans()
             launches, calls = [], self._plan_calls(self._own_grad, True)
         else:
             loose, launches, calls = set(), [], []           # launches: (p, g, m, v, group)
-            one_by_one = self._plans is None and capturing                # a plan's upload cannot be captured
+            one_by_one = capturing and (self._plans is None or self._moved())          # a plan's upload cannot be captured
             for group, runs in zip(self.param_groups, self._runs):
                 for run in runs:
                     if all(p.grad is None for p in run["params"]):
@@ -271,6 +279,8 @@ class AdamW(torch.optim.Optimizer):
                     self._refresh_plans()
                 # (betas as the single-tensor kernel takes them, in fp32: a tensor's update does not depend on which of the two serves it)
                 calls = self._plan_calls(lambda p: self._own_grad(p) if p in loose else None, False)
+        if capturing:
+            self._captured.append((self._step_dev, self._runs, [plan for plan, _, _ in calls]))
         check(lib().spn_adamw_tick(_p(self._step_dev), _p(found), _stream()), "adamw_tick")
         for p, g, m, v, group in launches:
             self._launch(p, g, m, v, group, scale, found)

@@ -75,3 +75,27 @@ def test_an_8_bit_first_step_under_capture_is_refused(optim):
             oa.step()
     oa.step(), ob.step()
     assert all(torch.equal(p, q) for p, q in zip(a, b)) and float(oa.state[a[0]]["step"]) == 1.0
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_loaded_state_leaves_an_older_graph_its_memory(optim, bits):
+    """A graph captured before load_state_dict() goes on with the moments, counter and tables it was captured with, whatever is allocated
+    afterwards; it is the twin that was never loaded."""
+    a, b = make(), make()
+    oa, ob = optim.AdamW(groups(a), state_bits=bits, **HP), optim.AdamW(groups(b), state_bits=bits, **HP)
+    for p, q, x in zip(a, b, gradients(a, 0)):
+        p.grad, q.grad = x.clone(), x.clone()
+    oa.step(), ob.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oa.step()
+    oa.load_state_dict(oa.state_dict())
+    junk = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in (64, 512, 1000, 4096, 20000, 100000) for _ in range(20)]
+    for _ in range(3):
+        torch.cuda.synchronize()
+        graph.replay()
+        ob.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    assert all(bool((t == 255).all()) for t in junk)

@@ -1,5 +1,8 @@
 """Host logic of spn4cir_amd.optim.AdamW on the CPU: the device calls are stand-ins that count and move the parameters by one."""
+import copy
+import gc
 import warnings
+import weakref
 
 import pytest
 import torch
@@ -169,3 +172,48 @@ def test_views_of_one_buffer_bump_the_buffer(device, bits):
         o.step()
         assert flat._version > before
     assert device.singles == (2 if bits == 32 else 0)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_what_a_captured_step_used_lives_on(device, bits):
+    """A graph holds addresses only: the plan (its table above all), the moments and the counter of a captured step survive a replaced p.data
+    and a loaded state."""
+    ps = make()
+    o = O.AdamW(ps, state_bits=bits, **HP)
+    o.step()
+    device.capturing = True
+    o.step()
+    device.capturing = False
+    plan, step, runs = weakref.ref(device.calls[-1][0]), o._step_dev.data_ptr(), o._runs
+    moments = weakref.ref(runs[0][0]["m"] if bits == 32 else plan().m)
+    del runs
+    device.calls.clear()
+    ps[1].data = ps[1].data.clone()
+    o.step()
+    assert device.calls[-1][0] is not plan()
+    o.load_state_dict(copy.deepcopy(o.state_dict()))
+    o.step()
+    device.calls.clear()
+    gc.collect()
+    assert plan() is not None and moments() is not None and o._captured[0][0].data_ptr() == step
+
+
+def test_a_capture_after_replaced_data(device):
+    """No plan is built inside a capture: 32 bits go tensor by tensor, 8 bits are refused."""
+    for bits in (32, 8):
+        device.capturing, device.singles = False, 0
+        ps = make()
+        o = O.AdamW(ps, state_bits=bits, **HP)
+        o.step()
+        n = len(device.calls)
+        ps[2].data = ps[2].data.clone()
+        device.capturing, device.fail = True, 1
+        if bits == 32:
+            o.step()
+            assert device.singles == 4 and len(device.calls) == n
+        else:
+            with pytest.raises(RuntimeError, match="one step"):
+                o.step()
+        device.capturing, device.fail = False, 0
+        o.step()
+        assert len(device.calls) == n + 1
