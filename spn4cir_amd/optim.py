@@ -161,8 +161,20 @@ class AdamW(torch.optim.Optimizer):
         self._runs, self._step_dev = all_runs, step_dev      # (last: a failed build is tried again by the next step)
 
     def load_state_dict(self, state_dict):
-        """torch semantics; the loaded per-parameter moments are copied into the flat state of the runs."""
-        super().load_state_dict(state_dict)
+        """torch semantics; the loaded per-parameter moments are copied into the flat state of the runs.  A state that is refused leaves the
+        optimizer as it was."""
+        kept = ("state", "param_groups", "_runs", "_plans", "_step_dev")
+        before = [getattr(self, name) for name in kept]
+        try:
+            super().load_state_dict(state_dict)
+            self._adopt()
+        except BaseException:
+            for name, value in zip(kept, before):
+                setattr(self, name, value)
+            raise
+
+    def _adopt(self):
+        """What torch has just put into self.state becomes the content of fresh runs or plans."""
         loaded = {p: dict(st) for p, st in self.state.items()}
         if self.state_bits == 8:
             self._load_8bit(loaded)

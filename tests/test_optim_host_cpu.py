@@ -217,3 +217,28 @@ def test_a_capture_after_replaced_data(device):
         device.capturing, device.fail = False, 0
         o.step()
         assert len(device.calls) == n + 1
+
+
+@pytest.mark.parametrize("bits,why", [(8, "other bits"), (32, "other bits"), (8, "size"), (32, "size"), (8, "memory")])
+def test_a_refused_state_changes_nothing(device, bits, why):
+    """A state of the other width, of another parameter's size, or one that finds no memory: the optimizer goes on with its own."""
+    ps, other = make(), make(5)[1:]
+    o, q = O.AdamW(ps, state_bits=bits, **HP), O.AdamW(make() if why != "size" else other, state_bits=40 - bits if why == "other bits" else bits, **HP)
+    o.step(), q.step()
+    sd = q.state_dict()
+    if why == "size":                                                # 8 bits: one more block of codes; 32 bits: as torch, one element more
+        for st in sd["state"].values():
+            st["exp_avg"] = torch.zeros(300)
+    sd["param_groups"][0]["lr"] = 5.0
+    state, groups = {p: dict(st) for p, st in o.state.items()}, o.param_groups
+    if why == "memory":
+        device.fail = 1
+    with pytest.raises((ValueError, RuntimeError)):
+        o.load_state_dict(sd)
+    assert o.param_groups is groups and groups[0]["lr"] == HP["lr"] and set(o.state) == set(state)
+    assert all(o.state[p][k] is t for p, st in state.items() for k, t in st.items())
+    o.step()
+    assert all(bool((p == 2).all()) for p in ps) and device.calls[-1][2][0]["lr"] == HP["lr"]
+    o.load_state_dict(copy.deepcopy(o.state_dict()))                 # and a state that fits is taken
+    o.step()
+    assert all(bool((p == 3).all()) for p in ps)
