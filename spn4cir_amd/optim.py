@@ -49,7 +49,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits: 8 or 32, not {state_bits!r}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         self.state_bits, self.seed = state_bits, int(seed)
-        self._plans = None                  # [(AdamWPlan, its parameters, its groups)]: 8-bit moments, or the tensors outside flat runs
+        self._plans = None                  # [(AdamWPlan, its parameters, the slice of its groups)]: 8-bit moments, or the tensors outside flat runs
         self._on_step = on_step             # e.g. model.parameters_changed (the models also notice the update themselves)
         self._runs = None                   # per group: [dict(params, p_flat, m, v, numel)]
         self._step_dev = None               # 0-dim fp32 device counter of APPLIED steps (shared by every state["step"])
@@ -57,8 +57,8 @@ class AdamW(torch.optim.Optimizer):
 
     # -------------------------------------------------------------------------------- layout
     def _make_plans(self, members):
-        """members: per group a list of (parameter, m, v) (moments None for 8 bits) -> [(AdamWPlan, its parameters, its groups)], one for
-        each 16 groups.  Parameters that share memory (tied weights held twice) are updated one after the other, each by a plan of its own.
+        """members: per group a list of (parameter, m, v) (moments None for 8 bits) -> [(AdamWPlan, its parameters, the slice of its
+        groups)], one for each 16 groups.  Parameters that share memory (tied weights held twice) are updated one after the other, each by a plan of its own.
         Nothing of the optimizer changes here: a plan that cannot be built (out of memory) leaves it as it was."""
         plans = []
         for g0 in range(0, len(members), ADAMW_GROUPS):
@@ -69,7 +69,7 @@ class AdamW(torch.optim.Optimizer):
             for some in ([t] for t in part) if tied else (part,):
                 state = None if self.state_bits == 8 else [(m, v) for _, (_, m, v) in some]
                 plan = AdamWPlan([p for _, (p, _, _) in some], state_bits=self.state_bits, groups=[i for i, _ in some], state=state)
-                plans.append((plan, [p for _, (p, _, _) in some], self.param_groups[g0:g0 + ADAMW_GROUPS]))
+                plans.append((plan, [p for _, (p, _, _) in some], slice(g0, g0 + ADAMW_GROUPS)))
         return plans
 
     def _build_8bit(self):
@@ -121,7 +121,7 @@ class AdamW(torch.optim.Optimizer):
             if all(g is None for g in grads):
                 continue
             calls.append((plan, grads, [dict(g, betas=g["betas"] if exact_betas else tuple(C.c_float(b).value for b in g["betas"]))
-                                        for g in groups]))
+                                        for g in self.param_groups[groups]]))
         return calls
 
     def _build_runs(self):

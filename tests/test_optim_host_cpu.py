@@ -242,3 +242,14 @@ def test_a_refused_state_changes_nothing(device, bits, why):
     o.load_state_dict(copy.deepcopy(o.state_dict()))                 # and a state that fits is taken
     o.step()
     assert all(bool((p == 3).all()) for p in ps)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_replaced_groups_count(device, bits):
+    """param_groups[i] = another dict after the first step (what a program that rebuilds its schedule does): the next step takes its values."""
+    ps = make()
+    o = O.AdamW([dict(params=ps[:2]), dict(params=ps[2:])], state_bits=bits, **HP)
+    o.step()
+    o.param_groups[1] = dict(o.param_groups[1], lr=0.5)
+    o.step()
+    assert [h["lr"] for h in device.calls[-1][2]] == [HP["lr"], 0.5]
