@@ -244,13 +244,25 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # launches go to the current stream of the parameters' device
+        di = next((p.get_device() for group in self.param_groups for p in group["params"]), -1)
+        if di >= 0 and di != torch.cuda.current_device():
+            with torch.cuda.device(di):
+                self._step()
+        else:
+            self._step()
+        if self._on_step is not None:
+            self._on_step()
+        return loss
+
+    def _step(self):
         capturing = torch.cuda.is_current_stream_capturing()
         if self._step_dev is None:
             if capturing and self.state_bits == 8:
                 raise RuntimeError("state_bits=8: call init_state() (or take one step) before step() is captured in a graph")
             if capturing:
                 warnings.warn("AdamW: the first step is being captured, so the graph zeroes the moments and the step counter too and every replay is a "
-                              "first step; call init_state() (or take one step) before the capture", stacklevel=4)
+                              "first step; call init_state() (or take one step) before the capture", stacklevel=5)
             self.init_state()
         scale = getattr(self, "grad_scale", None)          # set by torch.amp.GradScaler.step around this call
         found = getattr(self, "found_inf", None)
@@ -301,6 +313,3 @@ class AdamW(torch.optim.Optimizer):
         # the version counter of every parameter that was updated: autograd's check of saved tensors and the models, which re-derive their bf16
         # operands when it has moved, read it (parameters over one buffer need not share a counter)
         torch.autograd.graph.increment_version([p for group in self.param_groups for p in group["params"] if p.grad is not None and p in self.state])
-        if self._on_step is not None:
-            self._on_step()
-        return loss

@@ -253,3 +253,32 @@ def test_replaced_groups_count(device, bits):
     o.param_groups[1] = dict(o.param_groups[1], lr=0.5)
     o.step()
     assert [h["lr"] for h in device.calls[-1][2]] == [HP["lr"], 0.5]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_launches_go_to_the_parameters_device(device, bits, monkeypatch):
+    """Parameters on another device than the current one: every launch of the step, the counter's among them, finds theirs current."""
+    current, seen = [0], []
+
+    class Guard:
+        def __init__(self, di):
+            self.di = di
+
+        def __enter__(self):
+            self.old, current[0] = current[0], self.di
+
+        def __exit__(self, *args):
+            current[0] = self.old
+    monkeypatch.setattr(OnGpu, "get_device", lambda self: 3, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(O, "_stream", lambda: seen.append(current[0]))
+    real = device.multi
+    monkeypatch.setattr(O, "adamw_multi", lambda *a, **k: (seen.append(current[0]), real(*a, **k)))
+    flat, grad = torch.zeros(64), torch.ones(64)
+    ps = make(2) + [OnGpu(flat[i * 32:(i + 1) * 32]) for i in range(2)]
+    for i, p in enumerate(ps[2:]):
+        p.grad = grad[i * 32:(i + 1) * 32]
+    o = O.AdamW(ps, state_bits=bits, on_step=lambda: seen.append(-current[0]), **HP)
+    o.step()
+    assert seen == ([3, 3, 0] if bits == 8 else [3, 3, 3, 0])        # counter, (the flat run,) the plan; the callback sees the caller's device
