@@ -303,7 +303,8 @@ def quantize_fp8(x, block_rows=1, want="rows", colsum=False):
 
     want: "rows" = Fp8Blocks [R, C], blocks along each row; "cols" = Fp8Blocks of the TRANSPOSED matrix [C, R], blocks along R (what a
     product that reduces over R reads); "both" = (rows, cols) from one read of x.  block_rows=128: one scale for 128 x 128 values - the
-    two forms then hold the same codes (weights).  colsum=True appends the fp32 column sums [C] of x (a bias gradient)."""
+    two forms then hold the same codes (weights).  colsum=True appends the fp32 column sums [C] of x (a bias gradient).  A matrix without rows
+    has the rows form only."""
     if want not in ("rows", "cols", "both") or block_rows not in (1, 128):
         raise ValueError(f"quantize_fp8: want {want!r}, block_rows {block_rows!r}")
     di = x.get_device()
@@ -317,9 +318,12 @@ def quantize_fp8(x, block_rows=1, want="rows", colsum=False):
     else:
         typ, ld = _rows2d(x, "x")
         (R, Cn), xs, pitch, ptr = x.shape, None, 0, x.data_ptr()
-    if R == 0 or Cn == 0:
-        raise ValueError("quantize_fp8: empty matrix")
+    if Cn == 0 or (R == 0 and want != "rows"):
+        raise ValueError("quantize_fp8: no columns" if Cn == 0 else "quantize_fp8: the transpose of no rows has no blocks")
     dev = x.device
+    if R == 0:
+        q = Fp8Blocks.empty(0, Cn, dev)
+        return (q, torch.zeros(Cn, dtype=torch.float32, device=dev)) if colsum else q
     q = Fp8Blocks.empty(R, Cn, dev) if want != "cols" else None
     qt = Fp8Blocks.empty(Cn, R, dev) if want != "rows" else None
     cs = torch.empty(Cn, dtype=torch.float32, device=dev) if colsum else None
@@ -334,6 +338,23 @@ def quantize_fp8(x, block_rows=1, want="rows", colsum=False):
 @functools.lru_cache(maxsize=1024)          # a pure function of the shape (one part: gfx950)
 def _gemm_fp8_ws(M, N, K):
     return lib().spn_gemm_nt_fp8_workspace_bytes(M, N, K)
+
+
+def _product_out(out, M, N, dtype, accumulate, act, device):
+    """The output [M, N] of a product: the caller's or a new one -> (tensor, element type, row pitch)."""
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate=True needs out")
+        typ = _ELEM.get(dtype)
+        if typ is None:
+            raise ValueError(f"out_dtype: fp32, bf16 or fp16, not {dtype}")
+        return torch.empty(M, N, dtype=dtype, device=device), typ, N
+    if out.shape != (M, N):
+        raise ValueError(f"out: expected {(M, N)}, got {tuple(out.shape)}")
+    typ, ldc = _rows2d(out, "out", device.index)
+    if accumulate and (typ != 0 or act != ACT_NONE):
+        raise ValueError("accumulate=True needs an fp32 out and no activation")
+    return out, typ, ldc
 
 
 def gemm_nt_fp8(a, b, bias=None, act=ACT_NONE, out_dtype=torch.bfloat16, out=None, accumulate=False):
@@ -353,19 +374,7 @@ def gemm_nt_fp8(a, b, bias=None, act=ACT_NONE, out_dtype=torch.bfloat16, out=Non
     bp = None if bias is None else _vec(bias, N, "bias", di)
     if act not in (ACT_NONE, ACT_QUICKGELU, ACT_GELU_ERF):
         raise ValueError(f"act {act!r}")
-    if out is None:
-        if accumulate:
-            raise ValueError("accumulate=True needs out")
-        typ, ldc = _ELEM.get(out_dtype), N
-        if typ is None:
-            raise ValueError(f"out_dtype: fp32, bf16 or fp16, not {out_dtype}")
-        out = torch.empty(M, N, dtype=out_dtype, device=a.data.device)
-    else:
-        if out.shape != (M, N):
-            raise ValueError(f"out: expected {(M, N)}, got {tuple(out.shape)}")
-        typ, ldc = _rows2d(out, "out", di)
-        if accumulate and (typ != 0 or act != ACT_NONE):
-            raise ValueError("accumulate=True needs an fp32 out and no activation")
+    out, typ, ldc = _product_out(out, M, N, out_dtype, accumulate, act, a.data.device)
     if di < 0:
         _no_cpu()
     if M == 0:
@@ -389,7 +398,9 @@ def linear_fp8_fwd(x, w8, bias=None, w8_t=None, out_dtype=torch.bfloat16):
     if w8_t is None:
         x8 = x if isinstance(x, Fp8Blocks) else quantize_fp8(x)
         return gemm_nt_fp8(x8, w8, bias, out_dtype=out_dtype), None
-    if isinstance(x, Fp8Blocks):
+    if x.shape[0] == 0:                                      # an empty batch: no blocks along its rows
+        x8, x8_t = x if isinstance(x, Fp8Blocks) else quantize_fp8(x), None
+    elif isinstance(x, Fp8Blocks):
         x8, x8_t = x, quantize_fp8(x, want="cols")
     else:
         x8, x8_t = quantize_fp8(x, want="both")
@@ -402,6 +413,13 @@ def _linear_fp8_bwd(dy, saved, dx_dtype, dw_dtype, dw, accumulate):
     M, N = dy.shape
     if M != saved["M"] or N != saved["w8_t"].K:
         raise ValueError(f"dy {tuple(dy.shape)}: expected {(saved['M'], saved['w8_t'].K)}")
+    if M == 0:
+        _rows2d(dy, "dy", saved["w8_t"].get_device())
+        dw = _product_out(dw, N, saved["w8_t"].rows, dw_dtype, accumulate, ACT_NONE, dy.device)[0]
+        if not accumulate:
+            dw.zero_()
+        return (gemm_nt_fp8(Fp8Blocks.empty(0, N, dy.device), saved["w8_t"], out_dtype=dx_dtype), dw,
+                torch.zeros(N, dtype=torch.float32, device=dy.device) if saved["bias"] else None)
     if saved["bias"]:
         dy8, dy8_t, db = quantize_fp8(dy, want="both", colsum=True)
     else:

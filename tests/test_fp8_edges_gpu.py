@@ -1,0 +1,55 @@
+"""8-bit blocks at the edges: batches without rows."""
+import pytest
+import torch
+
+from test_fp8_gpu import rnd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from spn4cir_amd import ops as o
+    return o
+
+
+@pytest.mark.parametrize("form", ["numbers", "blocks"])
+def test_linear_of_an_empty_batch(ops, form):
+    """No rows: empty outputs, zero gradients of weight and bias (added to what is there with accumulate), in training and in serving."""
+    w8, w8_t = ops.quantize_fp8(rnd((130, 200), 1).cuda(), block_rows=128, want="both")
+    bias = rnd((130,), 2).cuda()
+    x = torch.zeros(0, 200, dtype=torch.bfloat16, device="cuda")
+    if form == "blocks":
+        x = ops.rmsnorm_fwd(x, torch.ones(200, device="cuda"), out_dtype="fp8")[0]
+    y, none = ops.linear_fp8_fwd(x, w8, bias)
+    assert none is None and y.shape == (0, 130) and y.dtype == torch.bfloat16
+    y, saved = ops.linear_fp8_fwd(x, w8, bias, w8_t=w8_t, out_dtype=torch.float32)
+    assert y.shape == (0, 130) and y.dtype == torch.float32
+    dy = torch.zeros(0, 130, device="cuda")
+    dx, dw, db = ops.linear_fp8_bwd(saved, dy, dx_dtype=torch.float16, dw_dtype=torch.bfloat16)
+    assert dx.shape == (0, 200) and dx.dtype == torch.float16
+    assert dw.shape == (130, 200) and dw.dtype == torch.bfloat16 and not dw.any() and db.shape == (130,) and not db.any()
+    into = torch.full((130, 207), 3.0, device="cuda")
+    assert ops.linear_fp8_bwd(saved, dy, dw=into[:, :200], accumulate=True)[1].data_ptr() == into.data_ptr() and bool((into == 3.0).all())
+    ops.linear_fp8_bwd(saved, dy, dw=into[:, :200])
+    assert not into[:, :200].any() and bool((into[:, 200:] == 3.0).all())
+    assert ops.linear_fp8_fwd(x, w8, w8_t=w8_t)[1]["bias"] is False
+    for bad in (dict(dw=torch.zeros(130, 199, device="cuda")), dict(accumulate=True), dict(dw_dtype=torch.int32),
+                dict(dw=torch.zeros(130, 200, dtype=torch.float16, device="cuda"), accumulate=True)):
+        with pytest.raises(ValueError):
+            ops.linear_fp8_bwd(saved, dy, **bad)
+    with pytest.raises(ValueError):
+        ops.linear_fp8_bwd(saved, torch.zeros(0, 131, device="cuda"))
+
+
+def test_quantize_without_rows(ops):
+    x = torch.zeros(0, 300, device="cuda")
+    q, cs = ops.quantize_fp8(x, colsum=True)
+    assert q.shape == (0, 300) and cs.shape == (300,) and not cs.any() and ops.quantize_fp8(q, block_rows=128).shape == (0, 300)
+    for bad in (dict(want="cols"), dict(want="both")):
+        with pytest.raises(ValueError, match="no rows"):
+            ops.quantize_fp8(x, **bad)
+    with pytest.raises(ValueError, match="no columns"):
+        ops.quantize_fp8(torch.zeros(3, 0, device="cuda"))
