@@ -252,6 +252,9 @@ class Fp8Blocks:
             raise ValueError("Fp8Blocks: codes must be 16-byte, scale bytes 4-byte aligned")
         _SET_DATA(self, data), _SET_SCALE(self, scale), _SET_K(self, K), _SET_ROWS(self, rows)
 
+    def __reduce__(self):                            # copies and pickles are built from their tensors, checks included
+        return Fp8Blocks, (self.data, self.scale, self.K)
+
     @property
     def shape(self):
         return torch.Size((self.rows, self.K))
