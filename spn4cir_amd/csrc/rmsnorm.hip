@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(const RmsArgs a) {
             float gf[8];
             to_f32(gm[i], gf);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * rs * gf[e];
+            for (int e = 0; e < 8; ++e) v[i][e] = (RAGGED ? c + e < a.W : c < a.W) ? v[i][e] * rs * gf[e] : 0.f;   // zero codes behind W, also where rs is NaN
             if (a.yt == ET_E4M3) {                         // uniform
                 const int sb = e4m3_block_byte(v[i]);
                 if (c < Wp) *(u32x2*)((uint8_t*)a.y + row * Wp + c) = e4m3_pack8(v[i], pow2_field(254 - sb));

@@ -1,4 +1,4 @@
-"""8-bit blocks at the edges: batches without rows."""
+"""8-bit blocks at the edges: batches without rows, padding behind a row of NaN."""
 import pytest
 import torch
 
@@ -53,3 +53,17 @@ def test_quantize_without_rows(ops):
             ops.quantize_fp8(x, **bad)
     with pytest.raises(ValueError, match="no columns"):
         ops.quantize_fp8(torch.zeros(3, 0, device="cuda"))
+
+
+@pytest.mark.parametrize("W", [1, 7, 120, 300, 520, 1001, 2056, 4100])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_codes_behind_a_row_of_nan_are_zero(ops, W, eps):
+    """rstd of a row is NaN (a NaN in it) or infinite (all zeros, eps = 0): the row's values are NaN, the codes behind them zero all the same."""
+    x = rnd((5, W), W)
+    x[1, W // 2] = float("nan")
+    x[2] = 0
+    x[3, 0] = float("inf")
+    y, _, rstd = ops.rmsnorm_fwd(x.cuda(), torch.ones(W, device="cuda"), eps=eps, out_dtype="fp8")
+    assert torch.isnan(rstd[1]) and (eps > 0 or torch.isinf(rstd[2]))
+    assert not y.data[:, W:].any()
+    assert bool((y.data[1, :W] & 0x7F == 0x7F).all()) and bool((y.data[2, :W] & 0x7F == (0x7F if eps == 0 else 0)).all())
