@@ -135,12 +135,13 @@ size_t spn_gemm_nt_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /* ---------------------------------------------------------------- RMSNorm
  * h = x + residual in the residual's type (fp32 or x's), rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * gamma; W <= 16384, rows of any
- * pitch >= W.  Squares are summed in fp32 (a sum past 3.4e38 gives rstd 0).  Without a residual (NULL) h is x itself and `h` is not written.  y_type SPN_E4M3: y and y_scale in the block format. */
+ * pitch >= W.  Squares are summed in fp32 (a sum past 3.4e38 gives rstd 0).  Without a residual (NULL) h is x itself and `h` is not written.  y_type SPN_E4M3: y (8-byte
+ * aligned) and y_scale in the block format. */
 int spn_rmsnorm_fwd(const void* x, int x_type, int64_t ldx, const void* residual, int r_type, int64_t ldr, const float* gamma, float eps,
                     void* h, void* y, int y_type, void* y_scale, float* rstd, int64_t rows, int W, void* stream);
 /* dx = rstd * (dy gamma - xh mean(dy gamma xh)) + dh, xh = h rstd (dh: gradient that reaches h directly, in h's type, or NULL); dx in h's
  * type, optionally a second copy dx2 in dx2_type; dgamma [W] = sum over rows of dy xh (overwritten).  Few rows need no ws (0 bytes).
- * dx and dx2 overlap none of the inputs. */
+ * ws 16-byte aligned.  dx and dx2 overlap none of the inputs. */
 int spn_rmsnorm_bwd(const void* dy, int dy_type, int64_t lddy, const void* h, int h_type, int64_t ldh, const float* gamma, const float* rstd,
                     const void* dh, int64_t lddh, void* dx, void* dx2, int dx2_type, float* dgamma, int64_t rows, int W, void* ws,
                     size_t ws_bytes, void* stream);

@@ -148,7 +148,7 @@ int rmsnorm_fwd(const RmsArgs& a, hipStream_t st) {
     if (a.rows < 0 || a.W <= 0 || !a.x || !a.gamma || !a.y || !a.rstd || (a.r && !a.h) || (a.yt == ET_E4M3 && !a.y_scale)) return SPN_ERR_ARG;
     if (a.W > RMS_MAX_W || a.ldx < a.W || (a.r && a.ldr < a.W)) return SPN_ERR_SHAPE;
     if (a.rows == 0) return SPN_OK;
-    if (a.yt < ET_F32 || a.yt > ET_E4M3 || a.xt < ET_F32 || a.xt > ET_F16) return SPN_ERR_ARG;
+    if (a.yt < ET_F32 || a.yt > ET_E4M3 || a.xt < ET_F32 || a.xt > ET_F16 || (a.yt == ET_E4M3 && (uintptr_t)a.y % 8)) return SPN_ERR_ARG;
     if (!a.r) {
         if (a.xt == ET_F32) return rms_fwd_launch<float, NoRes>(a, st);
         if (a.xt == ET_BF16) return rms_fwd_launch<bf16_t, NoRes>(a, st);
@@ -373,9 +373,9 @@ static int rms_bwd_launch(const RmsBwdArgs& args, hipStream_t st) {
 int rmsnorm_bwd(const RmsBwdArgs& a, hipStream_t st) {
     if (a.rows <= 0 || a.W <= 0 || !a.dy || !a.h || !a.gamma || !a.rstd || !a.dx || !a.dgamma) return SPN_ERR_ARG;
     if (a.W > RMS_MAX_W || a.lddy < a.W || a.ldh < a.W || (a.dh && a.lddh < a.W)) return SPN_ERR_SHAPE;
-    if (a.dyt < ET_F32 || a.dyt > ET_F16 || a.ht < ET_F32 || a.ht > ET_F16) return SPN_ERR_ARG;
+    if (a.dyt < ET_F32 || a.dyt > ET_F16 || a.ht < ET_F32 || a.ht > ET_F16 || (a.dx2 && (a.dx2t < ET_F32 || a.dx2t > ET_F16))) return SPN_ERR_ARG;
     const size_t need = rmsnorm_bwd_ws_bytes(a.rows, a.W);
-    if (need && (!a.ws || a.ws_bytes < need)) return SPN_ERR_WORKSPACE;
+    if (need && (!a.ws || a.ws_bytes < need || (uintptr_t)a.ws % 16)) return SPN_ERR_WORKSPACE;
     if (a.dyt == ET_F32) {
         if (a.ht == ET_F32) return rms_bwd_launch<float, float>(a, st);
         if (a.ht == ET_BF16) return rms_bwd_launch<float, bf16_t>(a, st);
