@@ -745,7 +745,8 @@ int gemm_nt_fp8(const Fp8Gemm& g, hipStream_t st) {
     if ((uintptr_t)g.a % 16 || (uintptr_t)g.b % 16 || (uintptr_t)g.sa % 4 || (uintptr_t)g.sb % 4) return SPN_ERR_SHAPE;
     if (g.out_type < ET_F32 || g.out_type > ET_F16 || (g.accumulate && (g.out_type != ET_F32 || g.act != ACT_NONE))) return SPN_ERR_ARG;
     if (g.act < ACT_NONE || g.act > ACT_GELU_ERF) return SPN_ERR_ARG;
-    if (g.ws_bytes < gemm_nt_fp8_ws_bytes(g.M, g.N, g.Kp) || (uintptr_t)g.ws % 16) return SPN_ERR_WORKSPACE;
+    const size_t need = gemm_nt_fp8_ws_bytes(g.M, g.N, g.Kp);
+    if (need && (!g.ws || g.ws_bytes < need || (uintptr_t)g.ws % 16)) return SPN_ERR_WORKSPACE;
     Fp8Tile p;
     p.a = g.a; p.b = g.b; p.sa = g.sa; p.sb = g.sb; p.M = g.M; p.N = g.N; p.Kp = g.Kp;
     p.pitch = qscale_pitch(g.Kp); p.nk = (int)(g.Kp / 128);

@@ -22,3 +22,10 @@ def test_rmsnorm_alignment_and_types(L):
     assert need > 0 and bwd(5000, OFF8, need) == WS and bwd(5000, ODD, need) == WS and bwd(5000, ONE, need - 1) == WS
     assert bwd(5000, ONE, need, ONE, 3) == ARG and bwd(5000, ONE, need, ONE, -1) == ARG and bwd(5000, ONE, need, ONE, 7) == ARG
     assert bwd(5000, ODD, need, None, 7) == WS                       # (no second copy: its type is not looked at)
+
+
+def test_product_workspace(L):
+    """Where k slices need one: not NULL, large enough, 16-byte aligned."""
+    g = lambda ws, nb: L.spn_gemm_nt_fp8(ONE, ONE, ONE, ONE, 2304, 768, 19712, None, 0, ONE, 1, 768, 0, ws, nb, None)  # noqa: E731
+    need = L.spn_gemm_nt_fp8_workspace_bytes(2304, 768, 19712)
+    assert need > 0 and g(None, need) == WS and g(ONE, need - 1) == WS and g(OFF8, need) == WS and g(None, 0) == WS
