@@ -263,6 +263,7 @@ int quantize_fp8(const QuantArgs& a, hipStream_t st) {
         case ET_F16: return quantize_launch<f16_t>(a, st);
         case ET_E4M3:
             if (!a.x_scale || a.ldx % 8 || (uintptr_t)a.x % 8) return SPN_ERR_ARG;
+            if (a.x_pitch < qblocks(a.C)) return SPN_ERR_SHAPE;
             return quantize_launch<E4m3In>(a, st);
         default: return SPN_ERR_ARG;
     }

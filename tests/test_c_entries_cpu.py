@@ -29,3 +29,9 @@ def test_product_workspace(L):
     g = lambda ws, nb: L.spn_gemm_nt_fp8(ONE, ONE, ONE, ONE, 2304, 768, 19712, None, 0, ONE, 1, 768, 0, ws, nb, None)  # noqa: E731
     need = L.spn_gemm_nt_fp8_workspace_bytes(2304, 768, 19712)
     assert need > 0 and g(None, need) == WS and g(ONE, need - 1) == WS and g(OFF8, need) == WS and g(None, 0) == WS
+
+
+def test_pitch_of_scale_bytes(L):
+    """Blocks that are quantised again: a row of scale bytes holds one for each block."""
+    for C_, pitch in ((128, 0), (129, 1), (1000, 7)):
+        assert L.spn_quantize_fp8(ONE, 3, 1024, ONE, pitch, 4, C_, 0, None, None, ONE, ONE, None, None, 0, None) == SHAPE
