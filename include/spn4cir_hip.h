@@ -122,7 +122,8 @@ size_t spn_layernorm_bwd_workspace_bytes(int rows, int W);
 int spn_quantize_fp8(const void* x, int type, int64_t ldx, const void* x_scale, int x_pitch, int64_t R, int64_t C, int square, void* q,
                      void* q_scale, void* qt, void* qt_scale, float* colsum, void* ws, size_t ws_bytes, void* stream);
 size_t spn_quantize_fp8_workspace_bytes(int64_t R, int64_t C);
-/* out [R, C] in out_type (SPN_F32 / SPN_BF16 / SPN_F16); bf16 and fp32 hold the stored values exactly */
+/* out [R, C] in out_type (SPN_F32 / SPN_BF16 / SPN_F16).  fp32 holds the stored values exactly up to its largest number (magnitudes from
+ * 248 * 2^120 on are stored as 2^128: infinity), bf16 too, but for blocks whose largest magnitude is below 2^-116 (steps under 2^-133 are rounded) */
 int spn_dequantize_fp8(const void* q, const void* scale, int64_t R, int64_t C, void* out, int out_type, void* stream);
 /* C[M, N] = act(A[M, K] . B[N, K]^T + bias) on two block-format operands (Kp = K rounded up to 128), fp32 accumulation, out fp32 / bf16 /
  * fp16 with row pitch ldc; accumulate = 1 adds into an fp32 output (no activation then).  F.linear with 8-bit operands

@@ -3,7 +3,7 @@
 // A block is 128 consecutive values along the axis a product reduces over.  amax = the largest finite magnitude, e = the smallest
 // whole number with amax <= 448 * 2^e (e >= -127), code = e4m3(x * 2^-e), scale byte = e + 127.  The scale is a power of two because
 // v_mfma_scale_f32_*_f8f6f4 multiplies by exactly such a byte per operand row inside the matrix pipe (no fp32 epilogue per block), because
-// a block then decodes exactly into bf16 (3 mantissa bits), and because a floating-point code's relative error does not depend on the
+// a block then decodes exactly into bf16 (3 mantissa bits; scale bytes 0..2 reach below its smallest number), and because a floating-point code's relative error does not depend on the
 // scale - only one binade of its 18 can be lost to the rounding of e.  Non-finite values become the NaN code and do not enter amax.
 #pragma once
 #include "common.h"

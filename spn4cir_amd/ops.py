@@ -275,7 +275,9 @@ class Fp8Blocks:
         return q
 
     def dequantize(self, dtype=torch.bfloat16):
-        """[rows, K] as numbers; fp32 and bf16 hold the stored values exactly."""
+        """[rows, K] as numbers.  fp32 holds the stored values exactly up to its largest number (magnitudes from 248 * 2^120 = 3.3e38 on are
+        stored as 2^128 and decode to infinity), bf16 too, but for blocks whose largest magnitude is below 2^-116, where what lies under
+        2^-133 is rounded."""
         return _dequantize_fp8(self, dtype)
 
 

@@ -1,8 +1,9 @@
-"""8-bit blocks at the edges: batches without rows, padding behind a row of NaN."""
+"""8-bit blocks at the edges: batches without rows, padding behind a row of NaN, the ends of the number range."""
 import pytest
 import torch
 
-from test_fp8_gpu import rnd
+from oracle import blocks8 as ob
+from test_fp8_gpu import rnd, same, values
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,25 @@ def test_codes_behind_a_row_of_nan_are_zero(ops, W, eps):
     assert torch.isnan(rstd[1]) and (eps > 0 or torch.isinf(rstd[2]))
     assert not y.data[:, W:].any()
     assert bool((y.data[1, :W] & 0x7F == 0x7F).all()) and bool((y.data[2, :W] & 0x7F == (0x7F if eps == 0 else 0)).all())
+
+
+def test_the_largest_and_smallest_numbers(ops):
+    """From 248 * 2^120 on (half way between two codes, ties to even) a magnitude is stored as 2^128: an infinity as a number, like bf16's own
+    rounding of it.  Scale bytes 0..2 reach below bf16's smallest number; fp32 holds all of it."""
+    top = 2.0 ** 120
+    x = torch.zeros(9, 128)
+    x[0, :4] = torch.tensor([torch.finfo(torch.float32).max, -torch.finfo(torch.float32).max, 1e38, 3.0])
+    x[1, :3] = torch.tensor([248.0 * top, 248.0 * top * (1 - 2.0 ** -24), -240.0 * top])
+    for b in range(4):                                               # largest magnitude 448 * 2^(b - 127): scale byte b; then down to the smallest code
+        x[2 + b] = torch.arange(128).double().mul(2.0 ** (b - 136)).float()
+        x[2 + b, 0] = 448.0 * 2.0 ** (b - 127)
+    x[6, 5], x[7, 5] = 2.0 ** -149, 2.0 ** -137                      # under half of the smallest code: zero; half of it: zero (even)
+    x[8] = torch.finfo(torch.float32).tiny
+    q = ops.quantize_fp8(x.cuda())
+    ref, e = ob.quantize(x)
+    assert same(values(q), ref) and torch.equal(q.scale.cpu()[:, :1].long() - 127, e.long())
+    assert ref[0, 0] == 2.0 ** 128 and ref[1, 0] == 2.0 ** 128 and ref[1, 1] == 240.0 * top and q.scale.cpu()[2:6, 0].tolist() == [0, 1, 2, 3]
+    full = q.dequantize(torch.float32).cpu()
+    assert torch.equal(full, ref.float()) and bool(torch.isinf(full[0, :2]).all()) and torch.equal(full[1:].double()[1:], ref[2:])
+    assert torch.equal(q.dequantize(torch.bfloat16).cpu(), ref.float().to(torch.bfloat16))
+    assert torch.equal(q.dequantize(torch.bfloat16).cpu()[5].double(), ref[5]) and not torch.equal(q.dequantize(torch.bfloat16).cpu()[2].double(), ref[2])
