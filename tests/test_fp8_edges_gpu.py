@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from oracle import blocks8 as ob
-from test_fp8_gpu import rnd, same, values
+from test_fp8_gpu import product, rnd, same, values
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,20 @@ def test_the_largest_and_smallest_numbers(ops):
     assert torch.equal(full, ref.float()) and bool(torch.isinf(full[0, :2]).all()) and torch.equal(full[1:].double()[1:], ref[2:])
     assert torch.equal(q.dequantize(torch.bfloat16).cpu(), ref.float().to(torch.bfloat16))
     assert torch.equal(q.dequantize(torch.bfloat16).cpu()[5].double(), ref[5]) and not torch.equal(q.dequantize(torch.bfloat16).cpu()[2].double(), ref[2])
+
+
+@pytest.mark.parametrize("M", [5, 40, 300])
+def test_product_at_the_ends_of_the_scale(ops, M):
+    """Scale bytes 0 to 4 of one operand against 236 to 247 of the other (in both orders): results of ordinary size, each kernel."""
+    N, K = 260, 640
+    g = torch.Generator().manual_seed(M)
+    mant = lambda r: torch.randn(r, K, generator=g).double().clamp(-3, 3) / 3  # noqa: E731
+    each = lambda r, lo, hi: torch.randint(lo, hi, (r, 5), generator=g).double().repeat_interleave(128, 1)  # noqa: E731
+    low = (mant(M) * 2.0 ** (each(M, 0, 4) - 118)).float()           # block maxima near 2^(b - 118): scale bytes 0..4
+    high = (mant(N) * 2.0 ** (each(N, 116, 124) + 1)).float()
+    a8, b8 = ops.quantize_fp8(low.cuda()), ops.quantize_fp8(high.cuda())
+    assert int(a8.scale.cpu()[:, :5].min()) == 0 and int(a8.scale.cpu()[:, :5].max()) <= 4 and int(b8.scale.cpu()[:, :5].max()) >= 240
+    ref, err = product(values(a8), values(b8))
+    for p, q, r in ((a8, b8, ref), (b8, a8, ref.t())):
+        got = ops.gemm_nt_fp8(p, q, out_dtype=torch.float32).cpu().double()
+        assert ((got - r).abs() <= (err if r is ref else err.t())).all()
