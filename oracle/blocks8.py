@@ -64,6 +64,7 @@ def adamw(p, g, m, v, t, lr, betas, eps, wd):
 
 
 def mix32(x):
+    """Two multiply-xorshift rounds; shifts and factors from Chris Wellons' published search for 32-bit integer hashes of low bias (2018)."""
     low = 0xFFFFFFFF
 
     def mul(a, k):                                   # 32 x 32 -> low 32 bits without leaving 63

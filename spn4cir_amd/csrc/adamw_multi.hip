@@ -8,9 +8,9 @@
 //
 // 8-bit moments, blocks of 128 with one byte of scale each: m as e4m3 (fp8.h), v as an UNSIGNED code of 5 exponent and 3 mantissa
 // bits - v spans the square of m's range, and an element whose v fell to 0 while its m did not would take a step of m / eps; a positive
-// v is never stored as 0.  Both are rounded stochastically with 16 random bits each from a hash of (seed, step, element index): v changes by at most
-// 0.1 % per step, rounding to nearest would drop every such change (half a step is 3-6 %) and the average would never decay.  The
-// update itself uses the unrounded moments in fp32.
+// v is never stored as 0.  Both are rounded stochastically with 16 random bits each from a hash of (seed, step, element index): where
+// gradients are small v falls by a share of 1 - b2 per step (0.1 % at b2 = 0.999); rounding to nearest would drop every change of less than half a
+// code's step (3-6 %), and the average would never decay.  The update itself uses the unrounded moments in fp32.
 //
 // Bound by HBM: 16 bytes per element with 8-bit moments and fp32 gradients, 28 with fp32 moments.  16 lanes hold a block of 128, so its scale is one DPP
 // reduction; chunks of 4 096 elements of one tensor are the unit of work, 4 workgroups per CU walk them (404 us below; 2: 410, 8: 402).
@@ -22,7 +22,8 @@ namespace spn {
 
 static constexpr int AM_CHUNK = 4096;          // elements of one tensor per work item
 
-// 32-bit mixing: two multiply-xorshift rounds, every input bit reaches every output bit
+// 32-bit mixing: two multiply-xorshift rounds, every input bit reaches every output bit.  Shifts and factors are from Chris Wellons' published search
+// for 32-bit integer hashes of low bias (2018).
 __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
     x = (x ^ (x >> 16)) * 0x7feb352du;
     x = (x ^ (x >> 15)) * 0x846ca68bu;
