@@ -50,11 +50,6 @@ class FusionLayout(C.Structure):
                [("bf16_off", C.c_int64 * 15)]
 
 
-class AdamwTensor(C.Structure):        # == spn_adamw_tensor
-    _fields_ = [(n, C.c_void_p) for n in ("p", "m", "v", "m_scale", "v_scale")] + \
-               [("n", C.c_int64), ("index0", C.c_int64), ("group", C.c_int32), ("pad", C.c_int32)]
-
-
 class AdamwGroup(C.Structure):         # == spn_adamw_group
     _fields_ = [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
 

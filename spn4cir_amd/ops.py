@@ -192,12 +192,6 @@ def _on_device(fn):
     return call
 
 
-def _elem(t, name):
-    if t.dtype not in _ELEM:
-        raise ValueError(f"{name}: expected fp32, bf16 or fp16, got {t.dtype}")
-    return _ELEM[t.dtype]
-
-
 def _rows2d(t, name, di=None):
     """A 2-D device tensor whose rows are contiguous, at any pitch >= the width -> (element type, row pitch); di: its device index."""
     typ = _ELEM.get(t.dtype)
