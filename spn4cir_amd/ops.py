@@ -1098,6 +1098,8 @@ class AdamWPlan:
 @_on_device
 def _adamw_moments(plan, dtype):
     m, v = (torch.empty(plan.total, dtype=dtype, device=plan.device) for _ in range(2))
+    if plan.total == 0:
+        return m, v
     check(lib().spn_adamw_moments(plan.m.data_ptr(), plan.m_scale.data_ptr(), plan.v.data_ptr(), plan.v_scale.data_ptr(), m.data_ptr(), v.data_ptr(),
                                   _ELEM[dtype], plan.total, _raw_stream(plan.get_device())), "adamw_moments")
     return m, v
@@ -1143,6 +1145,8 @@ def adamw_multi(plan, grads, step, hyper, seed=0, step_dev=None, inv_scale=1.0, 
         types = bytes([0 if g is None else _ELEM[g.dtype] for g in grads])
     groups = (_lib.AdamwGroup * len(hyper))(*[_lib.AdamwGroup(float(h["lr"]), float(h["betas"][0]), float(h["betas"][1]), float(h["eps"]),
                                                               float(h["weight_decay"])) for h in hyper])
+    if plan.total == 0:                                  # tensors without elements: nothing to launch
+        return
     check(lib().spn_adamw_multi(plan._table.data_ptr(), plan._chunks.data_ptr(), plan._prefix, ptrs.buffer_info()[0], types, n, groups, len(hyper),
                                 plan.state_bits, 0 if step_dev is not None else int(step), sp, float(inv_scale), gsp, fip, int(seed) & 0xFFFFFFFF,
                                 _raw_stream(di)), "adamw_multi")

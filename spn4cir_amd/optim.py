@@ -280,7 +280,7 @@ class AdamW(torch.optim.Optimizer):
             one_by_one = capturing and (self._plans is None or self._moved())          # a plan's upload cannot be captured
             for group, runs in zip(self.param_groups, self._runs):
                 for run in runs:
-                    if all(p.grad is None for p in run["params"]):
+                    if run["numel"] == 0 or all(p.grad is None for p in run["params"]):
                         continue
                     g = self._grads_flat(run) if len(run["params"]) > 1 else None
                     if g is not None:
@@ -289,7 +289,7 @@ class AdamW(torch.optim.Optimizer):
                         off = 0
                         for p in run["params"]:
                             g, n = p.grad, p.numel()
-                            if g is not None:
+                            if g is not None and n:
                                 launches.append((_flat_view(p, n), g.contiguous().float().view(-1), run["m"][off:off + n], run["v"][off:off + n],
                                                  group))
                             off += n

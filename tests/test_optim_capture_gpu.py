@@ -99,3 +99,28 @@ def test_a_loaded_state_leaves_an_older_graph_its_memory(optim, bits):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(a, b))
     assert all(bool((t == 255).all()) for t in junk)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("sizes", [(0,), (0, 0), (0, 5)])
+def test_parameters_without_elements(optim, bits, sizes):
+    """Alone, together and beside others; eager, and captured before any plan exists."""
+    from spn4cir_amd import ops
+    ps = [torch.nn.Parameter(torch.ones(n, device="cuda")) for n in sizes]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    plan = ops.AdamWPlan([p.data.clone() for p in ps], state_bits=bits)
+    ops.adamw_multi(plan, [p.grad for p in ps], 1, HP)
+    assert all(t.numel() == sum((n + 127) // 128 * 128 for n in sizes) for t in plan.moments())
+    o = optim.AdamW(ps, state_bits=bits, **HP)
+    o.init_state()
+    graph, other = torch.cuda.CUDAGraph(), torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        other.add_(1.0)
+        o.step()
+    o.step()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(o._step_dev) == 2.0 and all(bool((p < 1.0 - HP["lr"]).all()) for p in ps)
