@@ -39,6 +39,13 @@ def _flat_view(t, numel):
     return torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage(), t.storage_offset(), (numel,), (1,))
 
 
+def _counters(params):
+    """Parameters whose version counters cover all of theirs: one, if they are views of a tensor, else each."""
+    before = [p._version for p in params]
+    torch.autograd.graph.increment_version(params[:1])
+    return params[:1] if all(p._version > v for p, v in zip(params, before)) else params
+
+
 class AdamW(torch.optim.Optimizer):
     _step_supports_amp_scaling = True
 
@@ -51,7 +58,7 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.seed = state_bits, int(seed)
         self._plans = None                  # [(AdamWPlan, its parameters, the slice of its groups)]: 8-bit moments, or the tensors outside flat runs
         self._on_step = on_step             # e.g. model.parameters_changed (the models also notice the update themselves)
-        self._runs = None                   # per group: [dict(params, p_flat, m, v, numel)]
+        self._runs = None                   # per group: [dict(params, p_flat, m, v, numel, counters)]
         self._step_dev = None               # 0-dim fp32 device counter of APPLIED steps (shared by every state["step"])
         self._captured = []                 # what captured steps read and write: kept as long as the optimizer, their graphs hold addresses only
 
@@ -150,7 +157,7 @@ class AdamW(torch.optim.Optimizer):
                 n = sum(p.numel() for p in r)
                 m = torch.zeros(n, dtype=torch.float32, device=r[0].device)
                 v = torch.zeros(n, dtype=torch.float32, device=r[0].device)
-                out.append(dict(params=r, p_flat=_flat_view(r[0], n), m=m, v=v, numel=n))
+                out.append(dict(params=r, p_flat=_flat_view(r[0], n), m=m, v=v, numel=n, counters=None))
             all_runs.append(out)
         for run in (run for runs in all_runs for run in runs):
             off = 0
@@ -270,13 +277,14 @@ class AdamW(torch.optim.Optimizer):
             if t is not None and (t.dtype != torch.float32 or not t.is_cuda or t.numel() != 1):
                 raise TypeError("grad_scale / found_inf must be 1-element fp32 CUDA tensors")
         # everything that can fail for want of memory or a wrong layout is done before the step is counted and the first kernel launched
+        updated = []                                         # parameters, one at least for each version counter
         if self.state_bits == 8:
             if capturing and self._moved():
                 raise RuntimeError("state_bits=8: a parameter's data was replaced; take one step before step() is captured in a graph")
             self._refresh_plans()
             launches, calls = [], self._plan_calls(self._own_grad, True)
         else:
-            loose, launches, calls = set(), [], []           # launches: (p, g, m, v, group)
+            loose, launches, calls, pending = set(), [], [], []          # launches: (p, g, m, v, group)
             one_by_one = capturing and (self._plans is None or self._moved())          # a plan's upload cannot be captured
             for group, runs in zip(self.param_groups, self._runs):
                 for run in runs:
@@ -285,16 +293,29 @@ class AdamW(torch.optim.Optimizer):
                     g = self._grads_flat(run) if len(run["params"]) > 1 else None
                     if g is not None:
                         launches.append((run["p_flat"], g, run["m"], run["v"], group))
-                    elif one_by_one:
-                        off = 0
-                        for p in run["params"]:
-                            g, n = p.grad, p.numel()
-                            if g is not None and n:
-                                launches.append((_flat_view(p, n), g.contiguous().float().view(-1), run["m"][off:off + n], run["v"][off:off + n],
-                                                 group))
-                            off += n
-                    else:                                    # a tensor by itself, or gradients elsewhere: all such in one launch
-                        loose.update(run["params"])
+                        if run["counters"] is None:
+                            run["counters"] = _counters(run["params"])
+                        updated += run["counters"]
+                    else:                                    # a tensor by itself, or gradients elsewhere
+                        pending.append((run, group))
+            # one tensor alone goes through the single-tensor kernel (64 M elements: 350 us, in the many-tensor launch 369; 1000: 29 and 34 us of host
+            # time); several are faster together (4 x 16 M: 363 one by one, 368 together; 12 x 2 M: 190 and 142)
+            alone = len(pending) == 1 and len(pending[0][0]["params"]) == 1
+            for run, group in pending:
+                off = 0
+                if sum(map(torch.Tensor.numel, run["params"])) != run["numel"]:
+                    raise ValueError("a parameter changed its size after the first step")
+                for p in run["params"]:
+                    g, n = p.grad, p.numel()
+                    if not p.is_contiguous():
+                        raise TypeError("spn4cir_amd.optim.AdamW: parameters must be contiguous fp32 CUDA tensors")
+                    if g is not None and n:
+                        if one_by_one or (alone and g.dtype == torch.float32 and g.is_contiguous()):
+                            launches.append((_flat_view(p, n), g.contiguous().float().view(-1), run["m"][off:off + n], run["v"][off:off + n], group))
+                            updated.append(p)
+                        else:                                # all such in one launch
+                            loose.add(p)
+                    off += n
             if loose:
                 if self._plans is None:
                     self._plans = self._make_plans([[(p, self.state[p]["exp_avg"].view(-1), self.state[p]["exp_avg_sq"].view(-1)) for run in runs
@@ -312,4 +333,6 @@ class AdamW(torch.optim.Optimizer):
             adamw_multi(plan, grads, 0, hyper, seed=self.seed, step_dev=self._step_dev, grad_scale=scale, found_inf=found)
         # the version counter of every parameter that was updated: autograd's check of saved tensors and the models, which re-derive their bf16
         # operands when it has moved, read it (parameters over one buffer need not share a counter)
-        torch.autograd.graph.increment_version([p for group in self.param_groups for p in group["params"] if p.grad is not None and p in self.state])
+        for plan, grads, _ in calls:
+            updated += [p for p, g in zip(plan.params, grads) if g is not None]
+        torch.autograd.graph.increment_version(updated)

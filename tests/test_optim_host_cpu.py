@@ -76,7 +76,7 @@ def make(n=4):
 
 
 @pytest.mark.parametrize("bits", [8, 32])
-@pytest.mark.parametrize("groups,before", [(1, 1), (20, 1), (20, 2)])
+@pytest.mark.parametrize("groups,before", [(2, 1), (20, 1), (20, 2)])
 def test_a_failed_first_step_is_not_the_end(device, bits, groups, before):
     """The construction of the first or second of the plans raises once: that step counts nothing and updates nothing, the next one updates
     every parameter."""
@@ -282,3 +282,29 @@ def test_launches_go_to_the_parameters_device(device, bits, monkeypatch):
     o = O.AdamW(ps, state_bits=bits, on_step=lambda: seen.append(-current[0]), **HP)
     o.step()
     assert seen == ([3, 3, 0] if bits == 8 else [3, 3, 3, 0])        # counter, (the flat run,) the plan; the callback sees the caller's device
+
+
+def test_one_tensor_alone(device):
+    """32 bits: a single tensor needs no plan; a gradient of another type, or a second tensor, goes through one; its data may be replaced, but not by
+    another size, and not by columns of something wider."""
+    p, q = make(2)
+    q.grad = None
+    o = O.AdamW([p, q], **HP)
+    device.fail = 1
+    o.step()
+    assert device.singles == 1 and not device.calls and device.fail == 1
+    device.fail = 0
+    p.data = p.data.clone()
+    o.step()
+    assert device.singles == 2
+    q.grad = torch.ones(q.numel())
+    o.step()
+    assert device.singles == 2 and len(device.calls) == 1
+    q.grad = None
+    for data, error in ((torch.zeros(50), ValueError), (torch.zeros(5, 2)[:, 0], TypeError)):
+        p.grad, p.data = None, data
+        p.grad = torch.ones_like(data)
+        ticks = device.ticks
+        with pytest.raises(error):
+            o.step()
+        assert device.ticks == ticks and device.singles == 2 and len(device.calls) == 1
