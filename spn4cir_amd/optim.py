@@ -31,7 +31,7 @@ import warnings
 import torch
 
 from ._lib import check, lib
-from .ops import ADAMW_GROUPS, AdamWPlan, _p, _stream, adamw_multi, ranges_overlap
+from .ops import _DTYPE_OF, ADAMW_GROUPS, AdamWPlan, _p, _stream, adamw_multi, ranges_overlap
 
 
 def _flat_view(t, numel):
@@ -58,7 +58,7 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.seed = state_bits, int(seed)
         self._plans = None                  # [(AdamWPlan, its parameters, the slice of its groups)]: 8-bit moments, or the tensors outside flat runs
         self._on_step = on_step             # e.g. model.parameters_changed (the models also notice the update themselves)
-        self._runs = None                   # per group: [dict(params, p_flat, m, v, numel, counters)]
+        self._runs = None                   # per group: [dict(params, p_flat, m, v, numel, counters, addresses)]
         self._step_dev = None               # 0-dim fp32 device counter of APPLIED steps (shared by every state["step"])
         self._captured = []                 # what captured steps read and write: kept as long as the optimizer, their graphs hold addresses only
 
@@ -157,7 +157,8 @@ class AdamW(torch.optim.Optimizer):
                 n = sum(p.numel() for p in r)
                 m = torch.zeros(n, dtype=torch.float32, device=r[0].device)
                 v = torch.zeros(n, dtype=torch.float32, device=r[0].device)
-                out.append(dict(params=r, p_flat=_flat_view(r[0], n), m=m, v=v, numel=n, counters=None))
+                out.append(dict(params=r, p_flat=_flat_view(r[0], n), m=m, v=v, numel=n, counters=None,
+                                addresses=[p.data_ptr() for p in r]))
             all_runs.append(out)
         for run in (run for runs in all_runs for run in runs):
             off = 0
@@ -219,17 +220,20 @@ class AdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _grads_flat(run):
-        """The run's gradients as one flat tensor if they are consecutive slices of one buffer, else None."""
-        g0 = run["params"][0].grad
-        if g0 is None or g0.dtype != torch.float32 or not g0.is_contiguous():
+        """The run's gradients as one flat tensor if they are consecutive slices of one buffer and the parameters are where they were when the run was
+        laid out (p.data = ... moves them), else None."""
+        params, T = run["params"], torch.Tensor
+        grads = [p.grad for p in params]
+        g0 = grads[0]
+        if any(g is None for g in grads) or list(map(T.data_ptr, params)) != run["addresses"]:
             return None
-        base, off = g0.untyped_storage().data_ptr(), g0.storage_offset()
-        for p in run["params"]:
-            g = p.grad
-            if (g is None or g.dtype != torch.float32 or not g.is_contiguous() or g.device != p.device
-                    or g.untyped_storage().data_ptr() != base or g.storage_offset() != off):
-                return None
-            off += p.numel()
+        if set(map(_DTYPE_OF, grads)) != {torch.float32} or not all(map(T.is_contiguous, grads)) or g0.device != params[0].device:
+            return None
+        base, first = run["addresses"][0], g0.data_ptr()
+        if [x - first for x in map(T.data_ptr, grads)] != [x - base for x in run["addresses"]]:
+            return None
+        if g0.untyped_storage().nbytes() < 4 * (g0.storage_offset() + run["numel"]):       # neighbours by chance
+            return None
         return _flat_view(g0, run["numel"])
 
     # -------------------------------------------------------------------------------- step

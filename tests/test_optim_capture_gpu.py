@@ -124,3 +124,26 @@ def test_parameters_without_elements(optim, bits, sizes):
     graph.replay()
     torch.cuda.synchronize()
     assert float(o._step_dev) == 2.0 and all(bool((p < 1.0 - HP["lr"]).all()) for p in ps)
+
+
+def test_a_flat_run_whose_data_is_replaced(optim):
+    """Views of one buffer with their gradients in another; one view, then all of them, move: the bits of tensors that were always separate."""
+    def flat(seed):
+        buf, out, at = torch.zeros(sum(torch.Size(s).numel() for s in SHAPES), device="cuda"), [], 0
+        for p in make(seed):
+            out.append(buf[at:at + p.numel()].view(p.shape).copy_(p.detach()))
+            at += p.numel()
+        return out
+    a, b = [torch.nn.Parameter(x) for x in flat(0)], make()
+    g = flat(1)
+    for p, q, x in zip(a, b, g):
+        p.grad, q.grad = x, x.clone()
+    oa, ob = optim.AdamW(a, **HP), optim.AdamW(b, **HP)
+    for t in range(4):
+        if t == 1:
+            a[2].data = a[2].data.clone()
+        if t == 3:
+            for p, x in zip(a, flat(2)):
+                p.data = x.copy_(p.data)
+        oa.step(), ob.step()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), t

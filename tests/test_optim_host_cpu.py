@@ -308,3 +308,43 @@ def test_one_tensor_alone(device):
         with pytest.raises(error):
             o.step()
         assert device.ticks == ticks and device.singles == 2 and len(device.calls) == 1
+
+
+def test_a_flat_run_whose_data_is_replaced(device):
+    """One of the views of a flat buffer moves (p.data = a copy): the step goes to its new memory, the others to theirs; with all of them back in one
+    buffer the old one is left alone."""
+    flat, grad = torch.zeros(64), torch.ones(64)
+    ps = [OnGpu(flat[i * 16:(i + 1) * 16]) for i in range(4)]
+    for i, p in enumerate(ps):
+        p.grad = grad[i * 16:(i + 1) * 16]
+    o = O.AdamW(ps, **HP)
+    o.step()
+    assert device.singles == 1 and not device.calls
+    ps[2].data = ps[2].data.clone()
+    o.step()
+    assert device.singles == 1 and [p.data_ptr() for p in device.calls[-1][0].params] == [p.data_ptr() for p in ps]
+    other = torch.zeros(64)
+    for i, p in enumerate(ps):
+        p.data = other[i * 16:(i + 1) * 16]
+    o.step()
+    assert device.singles == 1 and bool((other == 1).all()) and len(device.calls) == 2
+
+
+def test_gradients_that_are_neighbours_by_chance(device):
+    """Consecutive addresses count only within one buffer; another order, a missing one and another type do not count either."""
+    flat, grad = torch.zeros(64), torch.ones(64)
+    ps = [OnGpu(flat[i * 16:(i + 1) * 16]) for i in range(4)]
+    o = O.AdamW(ps, **HP)
+
+    def step(grads):
+        for p, g in zip(ps, grads):
+            p.grad = g
+        before = device.singles
+        o.step()
+        return device.singles - before
+    whole = [grad[i * 16:(i + 1) * 16] for i in range(4)]
+    assert step(whole) == 1
+    assert step(whole[::-1]) == 0 and step(whole[:3] + [torch.ones(16)]) == 0 and step(whole[:3] + [None]) == 0
+    import numpy as np
+    raw = np.ones(64, np.float32)
+    assert step([torch.from_numpy(raw[i * 16:(i + 1) * 16]) for i in range(4)]) == 0          # four tensors that each own a part of it
