@@ -107,3 +107,12 @@ def test_product_at_the_ends_of_the_scale(ops, M):
     for p, q, r in ((a8, b8, ref), (b8, a8, ref.t())):
         got = ops.gemm_nt_fp8(p, q, out_dtype=torch.float32).cpu().double()
         assert ((got - r).abs() <= (err if r is ref else err.t())).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(4, 260, 4096), (300, 520, 640)])
+def test_full_fp32_sums_from_the_decoded_operands(ops, M, N, K):
+    """What a caller does who needs more than the 8-bit unit's 14 to 16 bits: bf16 holds the operands exactly, so K fp32 additions are all that rounds."""
+    a8, b8 = ops.quantize_fp8(rnd((M, K), 1).cuda()), ops.quantize_fp8(rnd((N, K), 2, scale=K ** -0.5).cuda(), block_rows=128)
+    a, b = values(a8), values(b8)
+    exact = ops.gemm_nt(a8.dequantize(), b8.dequantize(), out_dtype=torch.float32).cpu().double()
+    assert ((exact - a @ b.t()).abs() <= (K + 2) * 2.0 ** -24 * (a.abs() @ b.abs().t())).all()
