@@ -7,7 +7,7 @@
 // thread holds 8 rows x 8 columns), both scales come from it, the transposed codes turn through 16 KB of LDS so that both outputs leave
 // in whole 128-byte lines; the column sums (a bias gradient) ride along.
 // Measured: both forms of [8192, 8192] bf16 54 us, 5.0 TB/s; of [19712, 2304] with column sums 40 + 5.7 us (fold), 4.6 TB/s; square blocks of
-// fp32 [8192, 4096] 42 us, 4.8 TB/s; decoding [16384, 4096] to bf16 34 us, 6.0 TB/s.  A copy reaches 5.0.
+// fp32 [8192, 4096] 42 us, 4.8 TB/s; rows alone, [16384, 4096] bf16 34.9 us, 5.8 TB/s; stored blocks of that size along their columns 29.5 us, 4.6 TB/s; decoding [16384, 4096] to bf16 34 us, 6.0 TB/s.  A copy reaches 5.0.
 #include "fp8.h"
 #include "kernels.h"
 

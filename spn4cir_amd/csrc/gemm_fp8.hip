@@ -259,7 +259,8 @@ __device__ __forceinline__ int fp8_tile_of(const Fp8Tile& p, int bm, int bn, int
 // Measured cycles per k block (2048 of them matrix): 2 256; with stages of 64-byte half rows, where every 128-byte line is asked for twice,
 // 2 400-2 620; with 8 waves of 128 x 64 (192 KB out of LDS per k block) taking turns on the SIMDs, 2 720.  The epilogue takes 9 900 when one round of
 // tiles is all there is and up to 22 000 between rounds: all CUs store 33 MB at once, at the 4.6 TB/s a fill of that size reaches.
-// Bound by the power limit: 8192 x 8192 x 4096 in 219 us, 2.5 PFLOP/s, at 1.8 GHz (zeros as data: 20 % faster).
+// Bound by the power limit: 8192 x 8192 x 4096 in 217-222 us, 2.5 PFLOP/s, at 1.8 GHz (zeros as data: 20 % faster; in the first milliseconds of a load, while
+// the power management settles, up to 284).  fp32 outputs 248, with accumulate 310: twice the bytes stored, then as many read, behind the k loop.
 // Chunks behind the last k block are issued with an empty descriptor (zeros, no fetch), so the counts hold to the end.
 // Scales: two 4-byte DMA per lane and four k blocks bring the scale dwords of all 512 rows into one of two 2 KB buffers, four k blocks ahead; the
 // counted waits do not know of them, which makes the few that see them stricter, never laxer.

@@ -338,7 +338,8 @@ static int rms_bwd_blocks(int64_t rows, int W) {
 // Few rows of a matrix that stays in the caches: further workgroups of the same launch sum dgamma's columns from a second read - no partial rows,
 // no fold, no workspace, one launch (a call costs the host 9.1 instead of 13.1 us, which bounds it at these sizes).  A workgroup of 32 columns
 // reads 50 KB per us, so long columns lose.  On the GPU, columns / fold, us: 4 x 4096 3.1 / 5.7, 128 x 8192 4.2 / 10.2, 512 x 4096 4.5 / 14.2,
-// 1024 x 2048 6.1 / 10.6, 2048 x 1024 7.9 / 8.5 (bf16), 2048 x 768 (bf16, fp32 h) 10.8 / 8.7, 1237 x 1001 (fp16) 11.2 / 8.8; not taken: 2048 x 2048
+// 1024 x 2048 6.1 / 10.6, 2048 x 1024 7.9 / 8.5 (bf16), 2048 x 768 (bf16, fp32 h) 10.8 / 8.7, 1237 x 1001 (fp16) 11.2 / 8.8
+// (the last two lose 2 us where a graph replays them and the host does not count); not taken: 2048 x 2048
 // 14.7 / 12.7, 4096 x 512 12.3 / 7.8, 2048 x 8192 39 / 28.
 static bool rms_bwd_columns(int64_t rows, int W) { return rows <= 2048 && rows * W <= (1 << 21); }
 size_t rmsnorm_bwd_ws_bytes(int64_t rows, int W) {
