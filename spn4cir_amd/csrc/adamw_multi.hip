@@ -54,11 +54,14 @@ __device__ __forceinline__ void adamw_element(float& p, float g, float& m, float
 }
 
 // The same step where the moments are kept in 8 bits: square root and quotient by the one-ulp instructions (the moments' own rounding is
-// 2^-4 of a value; the exact forms cost a third of the kernel's vector instructions).  v below 2^-126 counts as 0 under the root.
+// 2^-4 of a value; the exact forms cost a third of the kernel's vector instructions).  The root instruction takes numbers below 2^-126 for 0, which
+// would divide m by eps alone: small v are brought up by 2^64 first.
 __device__ __forceinline__ void adamw_element8(float& p, float g, float& m, float& v, const AdamGroup& h, float decay, float step_size, float rsqrt_bc2) {
     m = __builtin_fmaf(h.omb1, g, h.b1 * m);
     v = __builtin_fmaf(h.b2, v, g * (h.omb2 * g));
-    const float denom = __builtin_fmaf(rsqrt_bc2, __builtin_amdgcn_sqrtf(v), h.eps);
+    const bool small = v < 0x1p-100f;
+    const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v);
+    const float denom = __builtin_fmaf(rsqrt_bc2, small ? root * 0x1p-32f : root, h.eps);
     p = __builtin_fmaf(decay, p, -(step_size * (m * __builtin_amdgcn_rcpf(denom))));
 }
 

@@ -51,3 +51,24 @@ def test_codes_flip_only_at_their_border(ops):
             expected = (2 * near.clamp(max=0.5) * one_scale).sum().item()
             assert int(flipped.sum()) <= expected + 6 * expected ** 0.5 + 6
             assert one_scale.double().mean() > 0.999
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-8])
+def test_second_moments_below_the_smallest_normal_number(ops, eps):
+    """Gradients of 1e-21 to 1e-17: v is subnormal, the step is lr * m / (sqrt(v) + eps) all the same, as with 32-bit moments.  v is off by at most 1.5 of
+    fp32's smallest step (two roundings of its terms), its root by half of that share, the rest by the few-ulp instructions."""
+    g = torch.Generator().manual_seed(1)
+    grad = torch.randn(4096, generator=g).sign() * 10.0 ** (torch.rand(4096, generator=g) * 4 - 21)
+    p0 = torch.randn(4096, generator=g)
+    h = dict(lr=1e-2, betas=(0.9, 0.999), eps=eps, weight_decay=0.0)
+    for bits in (8, 32):
+        p = p0.cuda()
+        ops.adamw_multi(ops.AdamWPlan([p], state_bits=bits), [grad.cuda()], 1, h)
+        zero = torch.zeros(4096)
+        ref, m, v = ob.adamw(p0, grad, zero, zero, 1, h["lr"], h["betas"], eps, 0.0)
+        share = 1.5 * 2.0 ** -149 / v                               # of v; where it is not small nothing is left of v's value
+        sure = share < 0.25
+        assert sure.double().mean() > 0.5 and (v < 2.0 ** -126).double().mean() > 0.3 and torch.isfinite(p.cpu()[sure]).all()
+        update = (ref - p0.double()).abs()
+        off = (p.cpu().double() - ref).abs()
+        assert (off <= update * (share + 2.0 ** -19) + 2.0 ** -22 * p0.double().abs())[sure].all(), bits
