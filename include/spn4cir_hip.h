@@ -136,7 +136,7 @@ size_t spn_gemm_nt_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /* ---------------------------------------------------------------- RMSNorm
  * h = x + residual in the residual's type (fp32 or x's), rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * gamma; W <= 16384, rows of any
- * pitch >= W.  Squares are summed in fp32 (a sum past 3.4e38 gives rstd 0).  Without a residual (NULL) h is x itself and `h` is not written.  y_type SPN_E4M3: y (8-byte
+ * pitch >= W.  Squares are summed in fp32 (a sum past 3.4e38 gives rstd 0, squares below 1e-45 vanish).  Without a residual (NULL) h is x itself and `h` is not written.  y_type SPN_E4M3: y (8-byte
  * aligned) and y_scale in the block format. */
 int spn_rmsnorm_fwd(const void* x, int x_type, int64_t ldx, const void* residual, int r_type, int64_t ldr, const float* gamma, float eps,
                     void* h, void* y, int y_type, void* y_scale, float* rstd, int64_t rows, int W, void* stream);

@@ -14,7 +14,7 @@
 //
 // Bound by HBM: 16 bytes per element with 8-bit moments and fp32 gradients, 28 with fp32 moments.  16 lanes hold a block of 128, so its scale is one DPP
 // reduction; chunks of 4 096 elements of one tensor are the unit of work, 4 workgroups per CU walk them (404 us below; 2: 410, 8: 402).
-// Measured: 123.65 M parameters in 150 tensors, 8 bits: 387-404 us, 4.9-5.1 TB/s (a copy: 5.0).  330 ragged tensors, 32 bits, bf16 gradients: 40 us.  Both moments decoded to bf16: 134 us.
+// Measured: 123.65 M parameters in 150 tensors, 8 bits: 387-407 us, 4.9-5.1 TB/s (a copy: 5.0).  330 ragged tensors, 32 bits, bf16 gradients: 40 us.  Both moments decoded to bf16: 134 us.
 #include "fp8.h"
 #include "kernels.h"
 

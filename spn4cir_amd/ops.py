@@ -444,7 +444,7 @@ def rmsnorm_fwd(x, gamma, residual=None, eps=1e-6, out_dtype=torch.bfloat16):
 
     x [rows, W] fp32 / bf16 / fp16 at any row pitch, W <= 16384, gamma fp32 [W]; without a residual h is x itself.  out_dtype: fp32 / bf16 /
     fp16, or "fp8": y as Fp8Blocks (one scale for 128 columns), ready for gemm_nt_fp8 / linear_fp8_fwd.  Squares are summed in fp32: a row whose
-    sum passes 3.4e38 (values near 1e18) gives rstd 0."""
+    sum passes 3.4e38 (values near 1e18) gives rstd 0, and one whose squares vanish (values below 1e-22) counts as zeros, which only eps = 0 shows."""
     xt, ldx = _rows2d(x, "x")
     rows, W = x.shape
     di, dev = x.get_device(), x.device

@@ -16,7 +16,8 @@ overflow itself - no `unscale_` pass over the gradients and no host synchronisat
 
 Parameters that are not part of such a flat run of several (or whose gradients are not the matching slices) are updated together by the
 many-tensor form of the same kernel (spn_adamw_multi: one launch, the same bits per tensor), so the class works for any fp32 CUDA
-parameter list; their gradients may be bf16 or fp16.
+parameter list; their gradients may be bf16 or fp16.  That launch's tables are built once (some 0.5 ms for 330 tensors) and again at a step
+that finds a parameter's data replaced.
 
 state_bits=8 keeps both moments in 8 bits (2.02 instead of 8 bytes per parameter; ops.AdamWPlan): all parameters of all groups go through
 spn_adamw_multi in one launch, whatever buffers they live in.  The moments are rounded stochastically by a hash of (seed, step, element),
