@@ -80,9 +80,14 @@ class AdamW(torch.optim.Optimizer):
                 plans.append((plan, [p for _, (p, _, _) in some], slice(g0, g0 + ADAMW_GROUPS)))
         return plans
 
+    def _device(self):
+        """The device of the first parameter that is trained (of the first one if none is)."""
+        every = lambda: (p for g in self.param_groups for p in g["params"])  # noqa: E731
+        return next((p for p in every() if p.requires_grad), next(every())).device
+
     def _build_8bit(self):
         ps = [[p for p in g["params"] if p.requires_grad] for g in self.param_groups]
-        dev = next(p.device for g in ps for p in g)
+        dev = self._device()
         for p in (p for g in ps for p in g):
             if p.dtype != torch.float32 or not p.is_cuda or not p.is_contiguous():
                 raise TypeError("spn4cir_amd.optim.AdamW: parameters must be contiguous fp32 CUDA tensors")
@@ -134,7 +139,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _build_runs(self):
         all_runs = []
-        dev = next(p.device for g in self.param_groups for p in g["params"])
+        dev = self._device()
         step_dev = torch.zeros((), dtype=torch.float32, device=dev)
         for group in self.param_groups:
             ps = [p for p in group["params"] if p.requires_grad]
@@ -257,8 +262,8 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         # launches go to the current stream of the parameters' device
-        di = next((p.get_device() for group in self.param_groups for p in group["params"]), -1)
-        if di >= 0 and di != torch.cuda.current_device():
+        di = self._device().index
+        if di is not None and di != torch.cuda.current_device():
             with torch.cuda.device(di):
                 self._step()
         else:

@@ -147,3 +147,15 @@ def test_a_flat_run_whose_data_is_replaced(optim):
                 p.data = x.copy_(p.data)
         oa.step(), ob.step()
         assert all(torch.equal(p, q) for p, q in zip(a, b)), t
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_frozen_parameter_in_front_elsewhere(optim, bits):
+    """A frozen parameter of another device (host memory) in front of the trained ones decides nothing."""
+    a, b = make(), make()
+    for p, q, x in zip(a, b, gradients(a, 0)):
+        p.grad, q.grad = x.clone(), x.clone()
+    frozen = torch.nn.Parameter(torch.ones(7), requires_grad=False)
+    oa, ob = optim.AdamW([frozen] + a, state_bits=bits, **HP), optim.AdamW(b, state_bits=bits, **HP)
+    oa.step(), ob.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and bool((frozen == 1).all()) and oa.state[a[0]]["step"].is_cuda

@@ -269,7 +269,9 @@ def test_launches_go_to_the_parameters_device(device, bits, monkeypatch):
 
         def __exit__(self, *args):
             current[0] = self.old
-    monkeypatch.setattr(OnGpu, "get_device", lambda self: 3, raising=False)
+    monkeypatch.setattr(O.AdamW, "_device", lambda self: torch.device("cuda", 3))
+    real_zeros = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, device=None, **k: real_zeros(*a, **k))
     monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
     monkeypatch.setattr(torch.cuda, "device", Guard)
     monkeypatch.setattr(O, "_stream", lambda: seen.append(current[0]))
@@ -348,3 +350,13 @@ def test_gradients_that_are_neighbours_by_chance(device):
     import numpy as np
     raw = np.ones(64, np.float32)
     assert step([torch.from_numpy(raw[i * 16:(i + 1) * 16]) for i in range(4)]) == 0          # four tensors that each own a part of it
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_nothing_to_train(device, bits):
+    ps = make()
+    for p in ps:
+        p.requires_grad_(False)
+    o = O.AdamW(ps, state_bits=bits, **HP)
+    o.step()
+    assert device.ticks == 1 and not device.calls and not any(bool(p.any()) for p in ps)
