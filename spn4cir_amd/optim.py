@@ -317,7 +317,9 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("a parameter changed its size after the first step")
                 for p in run["params"]:
                     g, n = p.grad, p.numel()
-                    if not p.is_contiguous():
+                    if g is not None and g.numel() != n:
+                        raise ValueError("a parameter changed its size after its gradient was computed")
+                    if p.dtype != torch.float32 or not p.is_cuda or not p.is_contiguous():
                         raise TypeError("spn4cir_amd.optim.AdamW: parameters must be contiguous fp32 CUDA tensors")
                     if g is not None and n:
                         if one_by_one or (alone and g.dtype == torch.float32 and g.is_contiguous()):

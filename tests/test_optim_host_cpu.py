@@ -360,3 +360,29 @@ def test_nothing_to_train(device, bits):
     o = O.AdamW(ps, state_bits=bits, **HP)
     o.step()
     assert device.ticks == 1 and not device.calls and not any(bool(p.any()) for p in ps)
+
+
+@pytest.mark.parametrize("capturing", [False, True])
+@pytest.mark.parametrize("what", ["type", "size"])
+def test_replaced_data_that_no_longer_fits(device, capturing, what):
+    """p.data of another type, or a gradient of another size than the data: refused before anything is launched, by itself and among others, also where
+    a capture goes tensor by tensor."""
+    for n in (1, 3):
+        device.capturing = False
+        ps = make(n)
+        o = O.AdamW(ps, **HP)
+        o.init_state()
+        p = ps[0]
+        if what == "type":
+            p.grad = None
+            p.data = p.data.half()
+            p.grad = torch.ones(p.numel(), dtype=torch.float16)
+        else:
+            data = p.data
+            p.data, p.grad = torch.zeros(3), None
+            p.grad = torch.ones(3)
+            p.data = data
+        device.capturing, ticks, singles, calls = capturing, device.ticks, device.singles, len(device.calls)
+        with pytest.raises((TypeError, ValueError)):
+            o.step()
+        assert (device.ticks, device.singles, len(device.calls)) == (ticks, singles, calls)
